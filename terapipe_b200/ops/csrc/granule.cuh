@@ -1,0 +1,57 @@
+// 16-byte pieces of rows of fp16, bf16 or fp32 as fp32 values, and rows found through strided outer indices.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "ptx.cuh"
+
+namespace tp {
+
+template <> struct Elem<float> {
+  __device__ static __forceinline__ float to_f(float v) { return v; }
+  __device__ static __forceinline__ float from_f(float v) { return v; }
+};
+
+template <typename T> struct Granule {
+  static constexpr int N = 16 / sizeof(T);
+  __device__ static __forceinline__ void unpack(const uint4& u, float (&f)[N]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 4) {
+        f[j] = __uint_as_float(w[j]);
+      } else {
+        const float2 t = Elem<T>::unpack2(w[j]);
+        f[2 * j] = t.x;
+        f[2 * j + 1] = t.y;
+      }
+    }
+  }
+  __device__ static __forceinline__ uint4 pack(const float (&f)[N]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 4) w[j] = __float_as_uint(f[j]);
+      else w[j] = Elem<T>::pack2(f[2 * j], f[2 * j + 1]);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+// Element offset of outer index i of an array [*, cols] of rows with strides s0 and s1: a batch-first array read in
+// sequence-first order needs no copy.
+struct OuterIndex {
+  long long s0, s1;
+  int cols;
+  __device__ __forceinline__ long long operator()(int i) const {
+    return cols == 1 ? i * s0 : (i / cols) * s0 + (i % cols) * s1;
+  }
+};
+
+// A whole number of an int32 or int64 array.
+__device__ __forceinline__ long long load_id(const void* p, long long i, int is64) {
+  return is64 ? static_cast<const long long*>(p)[i] : static_cast<const int*>(p)[i];
+}
+
+}  // namespace tp

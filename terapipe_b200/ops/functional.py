@@ -8,6 +8,7 @@ status word: call :func:`check_device_status` after a synchronisation point.
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Optional
 
 import torch
@@ -267,3 +268,243 @@ def attn_bwd(qkv, b: int, h: int, D: int, t: int, c: int, q_end: int, o, do_full
                                        _status_ptr(qkv), _stream())
     check(st, "tp_attn_bwd_scaled")
     return dqkv
+
+
+# ------------------------------------------------------------------ tokens in, losses out
+_DT_ROWS = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_DT_IDS = {torch.int32: 0, torch.int64: 1}
+MAX_TEACHER_ENTRIES = 1024
+
+
+def _kind(t: torch.Tensor, kinds, what: str) -> int:
+    code = kinds.get(t.dtype)
+    if code is None:
+        raise KernelError(f"{what}: unsupported dtype {t.dtype}")
+    return code
+
+
+def _same_device(*tensors) -> None:
+    """A pointer to another device's or the host's memory would be a fault in the kernel: it ends here."""
+    dev = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise KernelError(f"tensors of the current device cuda:{dev}, not {t.device}")
+
+
+def _outer(t: torch.Tensor, inner: int, n: int, what: str):
+    """``(columns, stride, stride)`` of the ``n`` outer indices of ``t`` before its last ``inner`` dimensions: of one or
+    two dimensions with any strides (a batch-first array seen sequence-first), or of more that a view can join."""
+    shape, st = t.shape, t.stride()
+    d = len(shape) - inner
+    if d < 0 or math.prod(shape[:d]) != n:
+        raise KernelError(f"{what} {tuple(shape)} does not have {n} rows")
+    if n <= 1:
+        return 1, 0, 0
+    if d == 2 and st[0] != shape[1] * st[1]:
+        return shape[1], st[0], st[1]
+    return 1, _joined(shape, st, d, what)[1], 0
+
+
+def _joined(shape, st, d: int, what: str):
+    """``(number, stride)`` of the first ``d`` dimensions as one."""
+    n, step = 1, 0
+    for k in range(d - 1, -1, -1):
+        if shape[k] == 1:
+            continue
+        if n == 1:
+            step = st[k]
+        elif st[k] != n * step and n:
+            raise KernelError(f"{what}: the first dimensions of {tuple(shape)} with strides {st} cannot be joined")
+        n *= shape[k]
+    return n, step
+
+
+def _matrix(t: torch.Tensor, what: str):
+    """``(rows, columns, row stride)`` of ``[..., columns]`` with contiguous columns and rows one stride apart."""
+    shape, st = t.shape, t.stride()
+    if not shape:
+        raise KernelError(f"{what} is a scalar")
+    rows, ld = (shape[0], st[0]) if len(shape) == 2 else _joined(shape, st, len(shape) - 1, what)
+    if st[-1] != 1 and shape[-1] > 1:
+        raise KernelError(f"{what}: columns are contiguous, not {st[-1]} apart")
+    if rows >= 2 ** 31 or shape[-1] >= 2 ** 31:
+        raise KernelError(f"{what}: {rows} rows of {shape[-1]} columns are too many")
+    return rows, shape[-1], ld
+
+
+def _written(t: torch.Tensor, rows: int, cols: int, ld: int, what: str) -> None:
+    if rows > 1 and cols and ld < cols:
+        raise KernelError(f"{what}: rows overlap")
+
+
+def embedding_fwd(ids, weight, out=None, *, scale: float = 1.0, first_row: int = 0):
+    """``out[i] = scale * weight[ids[i] - first_row]``: embedding rows of a batch of tokens.
+
+    ``ids`` (int32 or int64) have one or two dimensions with any strides, so a batch-first ``[batch, seq]`` array can be
+    passed transposed; ``out`` is ``[..., H]`` with a row per id, ``[*ids.shape, H]`` where it is left out.  ``weight`` is
+    fp16, bf16 or fp32 ``[rows, H]``: the whole table, or the rows from ``first_row`` on that a tensor-parallel rank
+    holds.  Ids in no row of it give zeros."""
+    n = ids.numel()
+    rows, H, ldw = _matrix(weight, "weight")
+    if out is None:
+        out = torch.empty(*ids.shape, H, dtype=weight.dtype, device=weight.device)
+    n_out, H_out, ldo = _matrix(out, "out")
+    if n_out != n or H_out != H or out.dtype != weight.dtype:
+        raise KernelError(f"out {tuple(out.shape)} {out.dtype} for {n} rows of {H} {weight.dtype}")
+    _written(out, n, H, ldo, "out")
+    _same_device(ids, weight, out)
+    cols, s0, s1 = _outer(ids, 0, n, "ids")
+    st = cuda_lib().tp_embedding_fwd(_kind(weight, _DT_ROWS, "weight"), ids.data_ptr(), _kind(ids, _DT_IDS, "ids"), n, cols,
+                                     s0, s1, first_row, weight.data_ptr(), ldw, rows, out.data_ptr(), ldo, H, scale,
+                                     _stream())
+    if st:
+        check(st, "tp_embedding_fwd")
+    return out
+
+
+def embedding_bwd_workspace_bytes(n: int, rows: int, H: int) -> int:
+    return cuda_lib().tp_embedding_bwd_workspace_blocks(int(n), int(rows), int(H)) * 256
+
+
+def embedding_bwd(ids, dy, dweight, *, scale: float = 1.0, first_row: int = 0, padding_id: Optional[int] = None,
+                  accumulate: bool = True, workspace=None):
+    """Gradient of :func:`embedding_fwd`: ``dweight[v] (+)= scale * sum of dy[i] with ids[i] - first_row == v``.
+
+    ``dy`` is fp16, bf16 or fp32 ``[..., H]``, ``dweight`` fp32 ``[rows, H]``.  Sums are formed in fp32 in an order that depends on the ids alone.
+    ``accumulate`` adds to what ``dweight`` holds and leaves the rows of absent tokens alone; without it they become
+    zero.  ``padding_id`` gets no gradient.  ``workspace``: :func:`embedding_bwd_workspace_bytes` bytes, allocated where
+    it is left out."""
+    n = ids.numel()
+    n_dy, H, ldy = _matrix(dy, "dy")
+    rows, H_w, ldw = _matrix(dweight, "dweight")
+    if n_dy != n or H_w != H:
+        raise KernelError(f"dy {tuple(dy.shape)} and dweight {tuple(dweight.shape)} for {n} ids")
+    if dweight.dtype != torch.float32:
+        raise KernelError(f"dweight is float32, not {dweight.dtype}")
+    _written(dweight, rows, H, ldw, "dweight")
+    lib = cuda_lib()
+    blocks = lib.tp_embedding_bwd_workspace_blocks(n, rows, H)
+    if workspace is None:
+        workspace = torch.empty(blocks * 256, dtype=torch.uint8, device=dweight.device)
+    elif workspace.numel() * workspace.element_size() < blocks * 256 or not workspace.is_contiguous() \
+            or workspace.data_ptr() % 16:
+        raise KernelError(f"workspace of {blocks * 256} contiguous bytes on a 16-byte boundary")
+    _same_device(ids, dy, dweight, workspace)
+    cols, s0, s1 = _outer(ids, 0, n, "ids")
+    st = lib.tp_embedding_bwd(_kind(dy, _DT_ROWS, "dy"), ids.data_ptr(), _kind(ids, _DT_IDS, "ids"), n, cols, s0, s1,
+                              first_row, -1 if padding_id is None else padding_id, dy.data_ptr(), ldy, dweight.data_ptr(),
+                              ldw, rows, H, scale, int(accumulate), workspace.data_ptr(), _stream())
+    if st:
+        check(st, "tp_embedding_bwd")
+    return dweight
+
+
+def _loss(mode, logits, teacher, labels, temperature, teacher_weight, ignore_id, loss=None, stats=None, dlogits=None,
+          grad_loss=None, grad_scale=1.0):
+    n, V, ld = _matrix(logits, "logits")
+    dtype = _kind(logits, _DT_ROWS, "logits")
+    label_args = (None, 0, 1, 0, 0, 0)
+    if labels is not None:
+        label_args = (labels.data_ptr(), _kind(labels, _DT_IDS, "labels"), *_outer(labels, 0, n, "labels"), ignore_id)
+    teacher_args = (None, 0, 1, 0, 0, None, 0, 1, 0, 0, 0)
+    tid = tlog = None
+    if teacher is not None:
+        tid, tlog = teacher
+        if tid.shape != tlog.shape or tid.dim() < 2:
+            raise KernelError(f"teacher ids {tuple(tid.shape)} and logits {tuple(tlog.shape)}: [..., entries] of one shape")
+        top = tid.shape[-1]
+        if top > MAX_TEACHER_ENTRIES:
+            raise KernelError(f"{top} teacher entries a row; at most {MAX_TEACHER_ENTRIES}")
+        if top > 1 and (tid.stride(-1) != 1 or tlog.stride(-1) != 1):
+            raise KernelError("a row's teacher entries are contiguous")
+        teacher_args = (tid.data_ptr(), _kind(tid, _DT_IDS, "teacher ids"), *_outer(tid, 1, n, "teacher ids"),
+                        tlog.data_ptr(), _kind(tlog, _DT_ROWS, "teacher logits"), *_outer(tlog, 1, n, "teacher logits"), top)
+        if not temperature > 0 or not 0 <= teacher_weight <= 1:
+            raise KernelError(f"temperature {temperature} is positive and teacher_weight {teacher_weight} in [0, 1]")
+    if mode & 1:
+        if loss is None:
+            loss = torch.empty(n, dtype=torch.float32, device=logits.device)
+        elif loss.dtype != torch.float32 or loss.numel() != n or not loss.is_contiguous():
+            raise KernelError(f"loss is float32 [{n}], contiguous")
+    if mode == 1 and stats is None:
+        stats = torch.empty(n, 4, dtype=torch.float32, device=logits.device)
+    elif stats is not None and (stats.dtype != torch.float32 or stats.numel() != 4 * n or not stats.is_contiguous()):
+        raise KernelError(f"stats is float32 [{n}, 4], contiguous")
+    ldd = ldg = 0
+    if mode & 2:
+        if dlogits is None:
+            dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        n_d, V_d, ldd = _matrix(dlogits, "dlogits")
+        if n_d != n or V_d != V or dlogits.dtype != logits.dtype:
+            raise KernelError(f"dlogits {tuple(dlogits.shape)} {dlogits.dtype} for logits {tuple(logits.shape)} {logits.dtype}")
+        _written(dlogits, n, V, ldd, "dlogits")
+        if n and V:
+            # in place, or apart: a row's gradient is stored while other rows' logits are still to be read
+            p, q, es = logits.data_ptr(), dlogits.data_ptr(), logits.element_size()
+            if (p != q or (ld != ldd and n > 1)) and p < q + ((n - 1) * ldd + V) * es and q < p + ((n - 1) * ld + V) * es:
+                raise KernelError("dlogits is logits itself or does not overlap it")
+        if grad_loss is not None:
+            if grad_loss.dtype != torch.float32:
+                raise KernelError(f"grad_loss is float32, not {grad_loss.dtype}")
+            n_g, ldg = _joined(grad_loss.shape, grad_loss.stride(), grad_loss.dim(), "grad_loss")
+            if n_g != n:
+                raise KernelError(f"grad_loss {tuple(grad_loss.shape)} does not have {n} rows")
+    _same_device(logits, labels, tid, tlog, loss, stats, dlogits, grad_loss)
+    st = cuda_lib().tp_loss(mode, dtype, logits.data_ptr(), ld, n, V, *label_args, *teacher_args, temperature,
+                            teacher_weight, _ptr(loss), _ptr(stats), _ptr(dlogits), ldd, _ptr(grad_loss), ldg, grad_scale,
+                            _stream())
+    if st:
+        check(st, "tp_loss")
+    return loss, stats, dlogits
+
+
+def distill_fwd(logits, teacher_ids, teacher_logits, labels=None, *, temperature: float = 1.0, teacher_weight: float = 1.0,
+                ignore_id: int = -100, loss=None, stats=None):
+    """Loss of every row of ``logits`` against a teacher's top logits; returns ``(loss, stats)``, fp32 ``[rows]`` and the
+    ``[rows, 4]`` that :func:`distill_bwd` needs.
+
+    ``loss = (1 - teacher_weight) * (logsumexp(z) - z[label]) + teacher_weight * T^2 * sum_k p_k (log p_k - log q[id_k])``
+    with ``p`` the softmax of the row's teacher logits divided by the temperature ``T`` and ``q`` that of ``z / T`` over the
+    whole vocabulary.
+
+    ``logits`` are fp16, bf16 or fp32 ``[..., vocabulary]``.  ``teacher_ids`` (int32 or int64) and ``teacher_logits`` (fp16,
+    bf16 or fp32) are ``[..., entries]`` with at most 1024 entries a row, in any order; an id outside the vocabulary (-1)
+    marks an absent entry, whose logit may be anything.  ``labels`` (int32 or int64) have an entry per row; both may be
+    transposed views.  A row whose label is ``ignore_id`` or outside the vocabulary has no first term, one without present
+    entries no second; with neither, or with all logits at -inf, it has the loss 0 and the gradient zero."""
+    return _loss(1, logits, (teacher_ids, teacher_logits), labels, temperature, teacher_weight, ignore_id, loss, stats)[:2]
+
+
+def distill_bwd(logits, stats, teacher_ids, teacher_logits, labels=None, *, temperature: float = 1.0,
+                teacher_weight: float = 1.0, ignore_id: int = -100, grad_loss=None, grad_scale: float = 1.0, dlogits=None):
+    """Gradient of :func:`distill_fwd`'s losses times ``grad_scale`` and, where given, ``grad_loss`` (fp32, a factor per
+    row).  ``dlogits`` has the type of ``logits`` and may be ``logits`` itself."""
+    return _loss(2, logits, (teacher_ids, teacher_logits), labels, temperature, teacher_weight, ignore_id, None, stats, dlogits,
+                 grad_loss, grad_scale)[2]
+
+
+def distill_fwd_bwd(logits, teacher_ids, teacher_logits, labels=None, *, temperature: float = 1.0,
+                    teacher_weight: float = 1.0, ignore_id: int = -100, grad_loss=None, grad_scale: float = 1.0, loss=None,
+                    dlogits=None):
+    """:func:`distill_fwd` and :func:`distill_bwd` with the logits read once: returns ``(loss, dlogits)``.  For a training
+    step, which knows the factor of every row's loss beforehand (loss scale over number of tokens)."""
+    loss, _, dlogits = _loss(3, logits, (teacher_ids, teacher_logits), labels, temperature, teacher_weight, ignore_id, loss,
+                             None, dlogits, grad_loss, grad_scale)
+    return loss, dlogits
+
+
+def cross_entropy_fwd(logits, labels, *, ignore_id: int = -100, loss=None, stats=None):
+    """``logsumexp(z) - z[label]`` of every row: :func:`distill_fwd` without a teacher."""
+    return _loss(1, logits, None, labels, 1.0, 0.0, ignore_id, loss, stats)[:2]
+
+
+def cross_entropy_bwd(logits, stats, labels, *, ignore_id: int = -100, grad_loss=None, grad_scale: float = 1.0, dlogits=None):
+    """Gradient of :func:`cross_entropy_fwd`, as :func:`distill_bwd`."""
+    return _loss(2, logits, None, labels, 1.0, 0.0, ignore_id, None, stats, dlogits, grad_loss, grad_scale)[2]
+
+
+def cross_entropy_fwd_bwd(logits, labels, *, ignore_id: int = -100, grad_loss=None, grad_scale: float = 1.0, loss=None,
+                          dlogits=None):
+    """:func:`cross_entropy_fwd` and :func:`cross_entropy_bwd` with the logits read once, as :func:`distill_fwd_bwd`."""
+    loss, _, dlogits = _loss(3, logits, None, labels, 1.0, 0.0, ignore_id, loss, None, dlogits, grad_loss, grad_scale)
+    return loss, dlogits
