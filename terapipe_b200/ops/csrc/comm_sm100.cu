@@ -418,12 +418,16 @@ TP_DEFINE_WAIT_LIMIT_SETTER(tp_set_wait_limit_ns_comm)
 extern "C" int tp_set_wait_limit_ns_gemm(unsigned long long ns);
 extern "C" int tp_set_wait_limit_ns_attn(unsigned long long ns);
 extern "C" int tp_set_wait_limit_ns_wgrad(unsigned long long ns);
+extern "C" int tp_set_wait_limit_ns_loss_fp16(unsigned long long ns);
+extern "C" int tp_set_wait_limit_ns_loss_bf16(unsigned long long ns);
+extern "C" int tp_set_wait_limit_ns_loss_fp32(unsigned long long ns);
 extern "C" int tp_set_wait_limit_ns(unsigned long long ns) {
   if (ns == 0) return kErrBadArgument;
   if (cudaDeviceSynchronize() != cudaSuccess) return kErrDriver;
   const int a = tp_set_wait_limit_ns_comm(ns), b = tp_set_wait_limit_ns_gemm(ns),
-            c = tp_set_wait_limit_ns_attn(ns), d = tp_set_wait_limit_ns_wgrad(ns);
-  return (a | b | c | d) ? kErrDriver : kOk;
+            c = tp_set_wait_limit_ns_attn(ns), d = tp_set_wait_limit_ns_wgrad(ns),
+            e = tp_set_wait_limit_ns_loss_fp16(ns), f = tp_set_wait_limit_ns_loss_bf16(ns), g = tp_set_wait_limit_ns_loss_fp32(ns);
+  return (a | b | c | d | e | f | g) ? kErrDriver : kOk;
 }
 
 // Which build this is: 1 when the kernels carry their index checks (-DTP_CHECKED), else 0.

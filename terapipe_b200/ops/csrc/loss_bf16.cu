@@ -1,0 +1,8 @@
+// The kernels of loss.cuh for bf16 logits (a file per type: they compile side by side).
+#include "loss.cuh"
+
+namespace tp {
+int loss_launch_bf16(const LossArgs& a, int mode, cudaStream_t s) { return loss_launch<__nv_bfloat16>(a, mode, s); }
+}  // namespace tp
+
+TP_DEFINE_WAIT_LIMIT_SETTER(tp_set_wait_limit_ns_loss_bf16)

@@ -419,8 +419,8 @@ def _loss(mode, logits, teacher, labels, temperature, teacher_weight, ignore_id,
             raise KernelError("a row's teacher entries are contiguous")
         teacher_args = (tid.data_ptr(), _kind(tid, _DT_IDS, "teacher ids"), *_outer(tid, 1, n, "teacher ids"),
                         tlog.data_ptr(), _kind(tlog, _DT_ROWS, "teacher logits"), *_outer(tlog, 1, n, "teacher logits"), top)
-        if not temperature > 0 or not 0 <= teacher_weight <= 1:
-            raise KernelError(f"temperature {temperature} is positive and teacher_weight {teacher_weight} in [0, 1]")
+        if not 2 ** -10 <= temperature <= 2 ** 10 or not 0 <= teacher_weight <= 1:
+            raise KernelError(f"temperature {temperature} in [2^-10, 2^10] and teacher_weight {teacher_weight} in [0, 1]")
     if mode & 1:
         if loss is None:
             loss = torch.empty(n, dtype=torch.float32, device=logits.device)
@@ -452,7 +452,7 @@ def _loss(mode, logits, teacher, labels, temperature, teacher_weight, ignore_id,
     _same_device(logits, labels, tid, tlog, loss, stats, dlogits, grad_loss)
     st = cuda_lib().tp_loss(mode, dtype, logits.data_ptr(), ld, n, V, *label_args, *teacher_args, temperature,
                             teacher_weight, _ptr(loss), _ptr(stats), _ptr(dlogits), ldd, _ptr(grad_loss), ldg, grad_scale,
-                            _stream())
+                            _status_ptr(logits), _stream())
     if st:
         check(st, "tp_loss")
     return loss, stats, dlogits
