@@ -60,47 +60,77 @@ embedding_fwd_kernel(const Tokens t, const T* __restrict__ w, long long ldw, T* 
 }
 
 // ------------------------------------------------------------------ tokens in the order of their rows
-// A stable radix sort by one cluster of 8 CTAs (the first of the grid), 256 warps that each own a contiguous piece of the tokens.  A pass counts
+// A stable radix sort of the tokens' rows by one cluster of 8 CTAs, 256 warps that each own a contiguous piece of the tokens.  A pass counts
 // the digits of every piece (one counter a digit and warp; lanes with the same digit are found by match_any and only the
 // first of them counts), turns the counts into destinations (digits, then CTAs, then warps) and moves keys and positions.
-// Equal keys keep their order, so that a row's sum does not depend on timing.  Tokens of no row get the key `rows` and
+// Equal keys keep their order, so that a row's sum does not depend on timing.  Tokens of no row have the key `rows` and
 // end up behind all others.
-constexpr int kSortCtas = 8, kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortBins = 512;
+constexpr int kSortCtas = 8, kSortMostCtas = 16, kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortBins = 512, kSortAhead = 8;
+constexpr int kSortMany = 16384;      // tokens from which on 16 CTAs sort: 147456 take 62 us instead of 97, up to 16384 either 15 to 20
 constexpr size_t kSortSmem = (kSortWarps * kSortBins + kSortBins + 2 * 32) * sizeof(int);
 
+// A token: its row (key) and its place in the batch.  One store of 8 bytes moves it: the scattered stores, 32 sectors a warp, are
+// what a pass over many tokens takes.
+using Token = uint2;      // x: key, y: place
+
 struct SortBuffers {
-  uint32_t *key[2], *pos[2];   // pass p writes [p & 1]
-  int passes, bits;            // digits a key, bits a digit
+  Token* at[2];       // pass p writes [p & 1]
+  int passes, bits;   // digits a key, bits a digit
 };
 
-__device__ void embedding_sort(const Tokens& t, const SortBuffers& b, int* sort_smem) {
+// Key of token i: its row, or `rows`.
+__device__ __forceinline__ uint32_t token_key(const Tokens& t, int i) {
+  const long long id = load_id(t.ids, t.at(i), t.is64), r = id - t.first;
+  return static_cast<uint32_t>(r >= 0 && r < t.rows && id != t.padding ? r : t.rows);
+}
+
+// seen[row] = some token of that row.  The array need not be cleared: row r occurs if seen[r] is a token whose row is r.
+__global__ void __launch_bounds__(256)
+embedding_mark_kernel(const Tokens t, uint32_t* __restrict__ seen) {
+  pdl_wait();
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= t.n) return;
+  const uint32_t k = token_key(t, i);
+  if (k < t.rows) seen[k] = i;
+}
+__device__ __forceinline__ bool row_occurs(const Tokens& t, const uint32_t* seen, long long r) {
+  const uint32_t i = __ldcg(seen + r);
+  return i < static_cast<uint32_t>(t.n) && token_key(t, static_cast<int>(i)) == static_cast<uint32_t>(r);
+}
+
+__global__ void __launch_bounds__(kSortThreads, 1)
+embedding_sort_kernel(const Tokens t, const SortBuffers b) {
+  extern __shared__ int sort_smem[];
+  const int n = t.n;
   int* hist = sort_smem;                              // [warp][bin]
   int* total = hist + kSortWarps * kSortBins;         // [bin], read by the other CTAs
   int* scan = total + kSortBins;                      // [32]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int cta = cluster_ctarank();
-  const int piece = ((t.n + kSortCtas * kSortWarps - 1) / (kSortCtas * kSortWarps) + 31) / 32 * 32;
+  const int cta = cluster_ctarank(), ctas = gridDim.x;      // (one cluster)
+  pdl_wait();
+  const int piece = ((n + ctas * kSortWarps - 1) / (ctas * kSortWarps) + 31) / 32 * 32;
   const long long begin = static_cast<long long>(cta * kSortWarps + warp) * piece;
-  const int lo = begin < t.n ? static_cast<int>(begin) : t.n;
-  const int hi = begin + piece < t.n ? static_cast<int>(begin) + piece : t.n;
+  const int lo = begin < n ? static_cast<int>(begin) : n;
+  const int hi = begin + piece < n ? static_cast<int>(begin) + piece : n;
   int* mine = hist + warp * kSortBins;
   for (int p = 0; p < b.passes; ++p) {
     const int shift = p * b.bits, bins = 1 << b.bits, digit_mask = bins - 1;
-    const uint32_t* key_in = b.key[(p + 1) & 1];
-    const uint32_t* pos_in = b.pos[(p + 1) & 1];
-    auto key_of = [&](int i) -> uint32_t {
-      if (p > 0) return __ldcg(key_in + i);
-      const long long id = load_id(t.ids, t.at(i), t.is64), r = id - t.first;
-      return r >= 0 && r < t.rows && id != t.padding ? static_cast<uint32_t>(r) : static_cast<uint32_t>(t.rows);
-    };
+    const Token* in_at = b.at[(p + 1) & 1];
     for (int d = lane; d < bins; d += 32) mine[d] = 0;
     __syncwarp();
-    for (int i = lo + lane; i - lane < hi; i += 32) {
-      const bool in = i < hi;
-      const int d = in ? (key_of(i) >> shift) & digit_mask : kSortBins;
-      const unsigned same = __match_any_sync(0xffffffffu, d);
-      if (in && lane == __ffs(same) - 1) mine[d] += __popc(same);
-      __syncwarp();
+    for (int i0 = lo + lane; i0 - lane < hi; i0 += 32 * kSortAhead) {
+      uint32_t key[kSortAhead];
+#pragma unroll
+      for (int k = 0; k < kSortAhead; ++k) key[k] = i0 + 32 * k >= hi ? 0 : p == 0 ? token_key(t, i0 + 32 * k) : __ldcg(&in_at[i0 + 32 * k].x);
+#pragma unroll
+      for (int k = 0; k < kSortAhead; ++k) {
+        if (i0 - lane + 32 * k >= hi) break;
+        const bool in = i0 + 32 * k < hi;
+        const int d = in ? (key[k] >> shift) & digit_mask : kSortBins;
+        const unsigned same = __match_any_sync(0xffffffffu, d);
+        if (in && lane == __ffs(same) - 1) mine[d] += __popc(same);
+        __syncwarp();
+      }
     }
     __syncthreads();
     if (tid < bins) {      // counts of the warps before each, and of the CTA
@@ -115,7 +145,7 @@ __device__ void embedding_sort(const Tokens& t, const SortBuffers& b, int* sort_
     cluster_sync_all();
     int before = 0, all = 0;
     if (tid < bins) {
-      for (int c = 0; c < kSortCtas; ++c) {
+      for (int c = 0; c < ctas; ++c) {
         int v;
         asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(mapa_u32(smem_u32(total + tid), c)) : "memory");
         before += c < cta ? v : 0;
@@ -135,69 +165,41 @@ __device__ void embedding_sort(const Tokens& t, const SortBuffers& b, int* sort_
       for (int w = 0; w < kSortWarps; ++w) hist[w * kSortBins + tid] += base;
     }
     __syncthreads();
-    for (int i = lo + lane; i - lane < hi; i += 32) {
-      const bool in = i < hi;
-      const uint32_t key = in ? key_of(i) : 0;
-      const int d = in ? (key >> shift) & digit_mask : kSortBins;
-      const unsigned same = __match_any_sync(0xffffffffu, d);
-      const int dest = in ? mine[d] + __popc(same & ((1u << lane) - 1)) : 0;
-      __syncwarp();
-      if (in) {
-        if (lane == __ffs(same) - 1) mine[d] += __popc(same);
-        __stcg(b.key[p & 1] + dest, key);
-        __stcg(b.pos[p & 1] + dest, p > 0 ? __ldcg(pos_in + i) : static_cast<uint32_t>(i));
+    for (int i0 = lo + lane; i0 - lane < hi; i0 += 32 * kSortAhead) {
+      Token v[kSortAhead];
+#pragma unroll
+      for (int k = 0; k < kSortAhead; ++k) v[k] = i0 + 32 * k >= hi ? make_uint2(0, 0) : p == 0 ? make_uint2(token_key(t, i0 + 32 * k), i0 + 32 * k) : __ldcg(in_at + i0 + 32 * k);
+#pragma unroll
+      for (int k = 0; k < kSortAhead; ++k) {
+        if (i0 - lane + 32 * k >= hi) break;
+        const bool in = i0 + 32 * k < hi;
+        const int d = in ? (v[k].x >> shift) & digit_mask : kSortBins;
+        const unsigned same = __match_any_sync(0xffffffffu, d);
+        const int dest = in ? mine[d] + __popc(same & ((1u << lane) - 1)) : 0;
+        __syncwarp();
+        if (in) {
+          if (lane == __ffs(same) - 1) mine[d] += __popc(same);
+          __stcg(b.at[p & 1] + dest, v[k]);
+        }
+        __syncwarp();
       }
-      __syncwarp();
     }
     __threadfence();
     cluster_sync_all();    // keys and positions are in place; no CTA reads this pass's totals any more
   }
 }
 
-// Zeros in the rows [begin, end) of the table that no token has: the CTA looks through all tokens and marks the rows that occur
-// in a bit map.  It needs nothing of the sort and runs beside it.
-__device__ void embedding_fill(const Tokens& t, long long begin, long long end, float* dw, long long ldw, int H, bool vec, uint32_t* map) {
-  const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5;
-  const int count = static_cast<int>(end - begin);
-  for (int i = tid; i < (count + 31) / 32; i += threads) map[i] = 0;
-  __syncthreads();
-  constexpr int kAhead = 8;
-  for (int i0 = tid; i0 < t.n; i0 += threads * kAhead) {
-    long long id[kAhead];
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int i = i0 + k * threads;
-      id[k] = i < t.n ? load_id(t.ids, t.at(i), t.is64) : t.padding;
-    }
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const long long r = id[k] - t.first - begin;
-      if (i0 + k * threads < t.n && r >= 0 && r < count && id[k] != t.padding) atomicOr(map + (r >> 5), 1u << (r & 31));
-    }
-  }
-  __syncthreads();
-  for (int r = warp; r < count; r += threads / 32) {
-    if (map[r >> 5] >> (r & 31) & 1) continue;
-    float* dst = dw + (begin + r) * ldw;
-    if (vec) {
-      for (int c = lane * 4; c < H; c += 128) *reinterpret_cast<float4*>(dst + c) = make_float4(0, 0, 0, 0);
-    } else {
-      for (int c = lane; c < H; c += 32) dst[c] = 0.0f;
-    }
-  }
-}
-
-// The first cluster sorts; with FILL the CTAs of the others write the zeros of `fill_rows` rows each.
-__global__ void __launch_bounds__(kSortThreads, 1)
-embedding_sort_kernel(const Tokens t, const SortBuffers b, float* dw, long long ldw, int H, int vec, int fill_rows) {
-  extern __shared__ int sort_smem[];
-  pdl_wait();
-  if (blockIdx.x < kSortCtas) {
-    embedding_sort(t, b, sort_smem);
+// ------------------------------------------------------------------ rows of absent tokens
+// Zeros in row r of the table, by a warp.
+__device__ __forceinline__ void zero_row(float* dw, long long ldw, long long r, int H, bool vec) {
+  const int lane = threadIdx.x & 31;
+  float* dst = dw + r * ldw;
+  if (vec) {
+#pragma unroll 4
+    for (int c = lane * 4; c < H; c += 128) *reinterpret_cast<float4*>(dst + c) = make_float4(0, 0, 0, 0);
   } else {
-    const long long begin = static_cast<long long>(blockIdx.x - kSortCtas) * fill_rows;
-    const long long end = begin + fill_rows < t.rows ? begin + fill_rows : t.rows;
-    if (begin < end) embedding_fill(t, begin, end, dw, ldw, H, vec, reinterpret_cast<uint32_t*>(sort_smem));
+#pragma unroll 4
+    for (int c = lane; c < H; c += 32) dst[c] = 0.0f;
   }
 }
 
@@ -215,7 +217,7 @@ template <typename T, bool VEC> struct Columns {
       constexpr int L = 8 * sizeof(T) / 16;
 #pragma unroll
       for (int i = 0; i < L; ++i)
-        if (c0 < H) v.u[i] = __ldg(reinterpret_cast<const uint4*>(row + c0) + i);
+        if (c0 < H) v.u[i] = __ldcs(reinterpret_cast<const uint4*>(row + c0) + i);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -269,19 +271,19 @@ struct SumArgs {
 
 enum { kHead = 1, kThrough = 2, kTail = 4 };
 
-// One CTA's chunk [lo, hi) of n sorted tokens, a piece of PIECE of them a warp, one block of columns.  A warp runs through its
-// rows of dy, eight of them under way, and stores a row's sum where the row's tokens all lie in its piece.  Of the others the
-// first (began in an earlier piece) and the last (goes on in the next) go to shared memory; then the warp in whose
+// One CTA's chunk [lo, hi) of n sorted tokens, a piece of at most 32 of them a warp, one block of columns.  A warp runs through its
+// rows of dy, a batch of them under way at a time, and stores a row's sum where the row's tokens all lie in its piece.  Of
+// the others the first (began in an earlier piece) and the last (goes on in the next) go to shared memory; then the warp in whose
 // piece a row began adds up the pieces in order.  Rows that cross the chunk's ends go to `part`.  So a token that
 // makes up a large share of the batch is summed by many warps, and always in the same order.
 template <typename T, bool VEC, int WARPS>
-__device__ void embedding_sums(const uint32_t* key, const uint32_t* pos, int n, int lo, int hi, int piece, int chunk, int block,
-                               const SumArgs& a, float (*slots)[2][256], int* flags) {
+__device__ void embedding_sums(const Token* tokens, int n, int lo, int hi, int piece, int chunk, int block, const SumArgs& a,
+                               float (*slots)[2][256], int* flags) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Columns<T, VEC> cols(block, lane, a.H);
   const T* dy = static_cast<const T*>(a.dy);
   const uint32_t none = static_cast<uint32_t>(a.rows);
-  const int p0 = min(lo + warp * piece, hi), p1 = min(p0 + piece, hi);
+  const int p0 = min(lo + warp * piece, hi), p1 = min(p0 + piece, hi), left = p1 - p0;
   int mark = 0;
   float acc[8] = {};
   uint32_t cur = none;
@@ -299,37 +301,35 @@ __device__ void embedding_sums(const uint32_t* key, const uint32_t* pos, int n, 
       mark |= kHead;
     }
   };
-  if (p0 < p1) {
-    const uint32_t before = p0 > 0 ? key[p0 - 1] : none;
-    constexpr int kAhead = 8;
-    for (int i = p0; i < p1; i += 32) {
-      const int left = min(32, p1 - i);
-      const uint32_t my_key = lane < left ? key[i + lane] : none, my_pos = lane < left ? pos[i + lane] : 0;
-      if (__shfl_sync(0xffffffffu, my_key, 0) == none) break;      // only tokens of no row from here on
-      for (int j0 = 0; j0 < left; j0 += kAhead) {
-        typename Columns<T, VEC>::Raw v[kAhead];
-        uint32_t k[kAhead];
+  if (left > 0) {
+    const uint32_t before = p0 > 0 ? tokens[p0 - 1].x : none, after = p1 < n ? tokens[p1].x : none;
+    constexpr int kBatch = sizeof(T) == 4 ? 4 : 8;
+    using Raw = typename Columns<T, VEC>::Raw;
+    const Token mine = lane < left ? tokens[p0 + lane] : make_uint2(none, 0);
+    for (int j0 = 0; j0 < left; j0 += kBatch) {
+      Raw v[kBatch];
+      uint32_t k[kBatch];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-          k[u] = __shfl_sync(0xffffffffu, my_key, j0 + u);
-          const uint32_t p = __shfl_sync(0xffffffffu, my_pos, j0 + u);
-          if (k[u] != none) cols.load(dy + p * a.ldy, v[u]);
+      for (int u = 0; u < kBatch; ++u) {
+        k[u] = __shfl_sync(0xffffffffu, mine.x, (j0 + u) & 31);
+        const uint32_t p = __shfl_sync(0xffffffffu, mine.y, (j0 + u) & 31);
+        if (k[u] != none) cols.load(dy + p * a.ldy, v[u]);
+      }
+      if (k[0] == none) break;      // only tokens of no row from here on
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        if (j0 + u >= left) break;
+        if (k[u] != cur || j0 + u == 0) {
+          finish();
+          began = j0 + u != 0 || before != k[u];
+          cur = k[u];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
         }
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-          if (j0 + u >= left) break;
-          if (k[u] != cur || (i == p0 && j0 + u == 0)) {
-            finish();
-            began = i != p0 || j0 + u != 0 || p0 == 0 || before != k[u];
-            cur = k[u];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
-          }
-          if (cur != none) cols.add(v[u], acc);
-        }
+        if (cur != none) cols.add(v[u], acc);
       }
     }
-    const bool goes_on = cur != none && p1 < n && key[p1] == cur;
+    const bool goes_on = cur != none && after == cur;
     if (!goes_on) {
       finish();
     } else if (began) {
@@ -367,36 +367,53 @@ __device__ void embedding_sums(const uint32_t* key, const uint32_t* pos, int n, 
   }
 }
 
-constexpr int kSumWarps = 8;
+// The first `fill` CTAs write the zeros of kZeroRows rows each, the others the sums.  Zeros need the marks only, which were there before the sort
+// began: the kernel starts as soon as the sort's 8 CTAs run, and only the CTAs with sums wait for these to end.  Many small CTAs,
+// as an SM writes about 40 GB/s at most: with a fixed share an SM, those beside the sort or with two shares took twice as
+// long as the others (50257 rows of 1600 columns: 84 us, 53 with one share on every SM, 47 with 8 rows a CTA).
+constexpr int kSumWarps = 8, kZeroRows = 16;
+
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kSumWarps * 32)
-embedding_sums_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ pos, int n, int piece, const SumArgs a) {
+__global__ void __launch_bounds__(kSumWarps * 32, 3)
+embedding_table_kernel(const Tokens t, const Token* __restrict__ tokens, const uint32_t* __restrict__ seen, int piece, int fill,
+                       int vec_fill, const SumArgs a) {
   __shared__ float slots[kSumWarps][2][256];
   __shared__ int flags[kSumWarps];
+  if (static_cast<int>(blockIdx.x) < fill) {
+    pdl_trigger();
+    // lane l of a warp looks whether row l of the CTA's occurs
+    const long long r0 = static_cast<long long>(blockIdx.x) * kZeroRows;
+    const int lane = threadIdx.x & 31;
+    const unsigned absent = __ballot_sync(0xffffffffu, lane < kZeroRows && r0 + lane < a.rows && !row_occurs(t, seen, r0 + lane));
+#pragma unroll
+    for (int k = threadIdx.x >> 5; k < kZeroRows; k += kSumWarps)
+      if (absent >> k & 1) zero_row(a.dw, a.ldw, r0 + k, a.H, vec_fill);
+    return;
+  }
   pdl_wait();
-  const int chunk = blockIdx.x / a.blocks, block = blockIdx.x % a.blocks, lo = chunk * piece * kSumWarps;
-  embedding_sums<T, VEC, kSumWarps>(key, pos, n, lo, min(lo + piece * kSumWarps, n), piece, chunk, block, a, slots, flags);
+  const int item = blockIdx.x - fill, chunk = item / a.blocks, block = item % a.blocks, lo = chunk * piece * kSumWarps;
+  embedding_sums<T, VEC, kSumWarps>(tokens, t.n, lo, min(lo + piece * kSumWarps, t.n), piece, chunk, block, a, slots, flags);
 }
 
 // Rows that cross ends of chunks: a warp per chunk and block of columns adds up, in order, the row that begins in its chunk and
 // goes on in the next.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256)
-embedding_join_kernel(const uint32_t* __restrict__ key, int n, int length, int chunks, const SumArgs a) {
+__global__ void __launch_bounds__(512)
+embedding_join_kernel(const Token* __restrict__ tokens, int n, int length, int chunks, const SumArgs a) {
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const long long item = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const long long item = static_cast<long long>(blockIdx.x) * 16 + (threadIdx.x >> 5);
   const int chunk = static_cast<int>(item / a.blocks), block = static_cast<int>(item % a.blocks);
   const long long next = static_cast<long long>(chunk + 1) * length;      // first token of the next chunk
   if (next >= n) return;
-  const uint32_t k = key[next];
-  if (k == static_cast<uint32_t>(a.rows) || key[next - 1] != k || (chunk > 0 && key[next - length - 1] == k)) return;
+  const uint32_t k = tokens[next].x;
+  if (k == static_cast<uint32_t>(a.rows) || tokens[next - 1].x != k || (chunk > 0 && tokens[next - length - 1].x == k)) return;
   // the last chunk of the row: the first whose own last token is another's
   int last = chunk + 1;
   while (true) {
     const long long e = static_cast<long long>(last + lane + 1) * length;      // end of chunk last + lane
-    const unsigned more = __ballot_sync(0xffffffffu, e < n && key[e] == k);
+    const unsigned more = __ballot_sync(0xffffffffu, e < n && tokens[e].x == k);
     if (more != 0xffffffffu) {
       last += __ffs(~more) - 1;
       break;
@@ -409,10 +426,17 @@ embedding_join_kernel(const uint32_t* __restrict__ key, int n, int length, int c
   for (int j = 0; j < 8; ++j) acc[j] = p[j * 32];
   p += a.blocks * 256;      // [chunk + 1][0]
   const long long step = 2ll * a.blocks * 256;
-#pragma unroll 4
-  for (int c = chunk + 1; c <= last; ++c, p += step) {
+  constexpr int kAhead = 8;      // chunks whose sums are under way
+  for (int c = chunk + 1; c <= last; c += kAhead, p += kAhead * step) {
+    float v[kAhead][8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] += p[j * 32];
+    for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[u][j] = c + u <= last ? p[u * step + j * 32] : 0.0f;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] += v[u][j];
   }
   const Columns<T, VEC> cols(block, lane, a.H);
   cols.write(a.dw + k * a.ldw, acc, a.scale, a.accumulate);
@@ -425,15 +449,24 @@ constexpr int kFewTokens = 512, kFewWarps = 16;
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kFewWarps * 32)
-embedding_few_kernel(const Tokens t, const SumArgs a, int vec_fill, int fill_rows) {
+embedding_few_kernel(const Tokens t, const SumArgs a, int vec_fill, int zero_rows) {
   __shared__ __align__(16) uint32_t raw[kFewTokens];
-  __shared__ uint32_t key[kFewTokens], pos[kFewTokens];
+  __shared__ Token tokens[kFewTokens];
   __shared__ float slots[kFewWarps][2][256];
   __shared__ int flags[kFewWarps];
   pdl_wait();
-  if (static_cast<int>(blockIdx.x) >= a.blocks) {
-    const long long begin = static_cast<long long>(blockIdx.x - a.blocks) * fill_rows;
-    embedding_fill(t, begin, min(begin + fill_rows, t.rows), a.dw, a.ldw, a.H, vec_fill, reinterpret_cast<uint32_t*>(slots));
+  if (static_cast<int>(blockIdx.x) >= a.blocks) {      // zeros in the rows [begin, end)
+    const long long begin = static_cast<long long>(blockIdx.x - a.blocks) * zero_rows, end = min(begin + zero_rows, a.rows);
+    uint32_t* map = reinterpret_cast<uint32_t*>(slots);
+    for (int i = threadIdx.x; i < (zero_rows + 31) / 32; i += kFewWarps * 32) map[i] = 0;
+    __syncthreads();
+    if (threadIdx.x < t.n) {
+      const long long id = load_id(t.ids, t.at(threadIdx.x), t.is64), r = id - t.first;
+      if (r >= begin && r < end && id != t.padding) atomicOr(map + ((r - begin) >> 5), 1u << ((r - begin) & 31));
+    }
+    __syncthreads();
+    for (long long r = begin + (threadIdx.x >> 5); r < end; r += kFewWarps)
+      if (!(map[(r - begin) >> 5] >> ((r - begin) & 31) & 1)) zero_row(a.dw, a.ldw, r, a.H, vec_fill);
     return;
   }
   const int i = threadIdx.x, padded = (t.n + 3) / 4 * 4;
@@ -451,11 +484,10 @@ embedding_few_kernel(const Tokens t, const SumArgs a, int vec_fill, int fill_row
       place += (k.x < mine || (k.x == mine && j < i)) + (k.y < mine || (k.y == mine && j + 1 < i)) +
                (k.z < mine || (k.z == mine && j + 2 < i)) + (k.w < mine || (k.w == mine && j + 3 < i));
     }
-    key[place] = mine;
-    pos[place] = i;
+    tokens[place] = make_uint2(mine, i);
   }
   __syncthreads();
-  embedding_sums<T, VEC, kFewWarps>(key, pos, t.n, 0, t.n, (t.n + kFewWarps - 1) / kFewWarps, 0, blockIdx.x, a, slots, flags);
+  embedding_sums<T, VEC, kFewWarps>(tokens, t.n, 0, t.n, (t.n + kFewWarps - 1) / kFewWarps, 0, blockIdx.x, a, slots, flags);
 }
 
 static bool make_tokens(Tokens* t, const void* ids, int ids64, int n, int cols, long long s0, long long s1, long long first,
@@ -487,10 +519,53 @@ static int key_bits(long long rows) {   // keys are 0 .. rows
 // Tokens a warp sums: 32 where that leaves 32 warps for every SM, else 8.  5105 tokens of 1600 columns: PIECE8 us against PIECE32.
 static int sum_piece(int n, int H) { return static_cast<long long>(n) * ((H + 255) / 256) >= 32ll * 32 * num_sms() ? 32 : 8; }
 
-// Rows a CTA of `ctas` fills, at most what its bit map (of `bits`) holds.
-static int fill_rows_of(long long rows, int ctas, int bits) {
-  const long long r = (rows + ctas - 1) / ctas;
-  return static_cast<int>(r < bits ? r : bits);
+
+// CTAs of the sort: 8, for many tokens 16 where the device runs a cluster of so many.  0: the kernel cannot be launched.
+static int sort_cluster(int n) {
+  struct Device {
+    bool ready;
+    int most;
+  };
+  static Device known[16];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  Device& d = known[dev & 15];
+  if (!d.ready) {
+    if (cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortSmem) != cudaSuccess) return 0;
+    d.most = kSortCtas;
+    if (cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute attr[1];
+      cfg.gridDim = dim3(kSortMostCtas);
+      cfg.blockDim = dim3(kSortThreads);
+      cfg.dynamicSmemBytes = kSortSmem;
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = kSortMostCtas;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int fit = 0;
+      if (cudaOccupancyMaxActiveClusters(&fit, embedding_sort_kernel, &cfg) == cudaSuccess && fit > 0) d.most = kSortMostCtas;
+    }
+    (void)cudaGetLastError();      // (of a size that does not fit)
+    d.ready = true;
+  }
+  return n >= kSortMany ? d.most : kSortCtas;
+}
+
+// launch_pdl for a kernel of any size that is meant to run beside the one before it.
+template <typename... KArgs, typename... Args>
+static bool launch_beside(void (*kern)(KArgs...), unsigned grid, unsigned block, cudaStream_t s, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.stream = s;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...) == cudaSuccess;
 }
 
 template <typename T, bool VEC>
@@ -498,41 +573,32 @@ static int embedding_bwd_launch(const Tokens& t, const SumArgs& args, uint32_t* 
   SumArgs a = args;
   const int vec_fill = a.H % 4 == 0 && a.ldw % 4 == 0 && (reinterpret_cast<uintptr_t>(a.dw) & 15) == 0;
   if (t.n <= kFewTokens) {
-    const int fill_rows = fill_rows_of(t.rows, 2 * num_sms(), kFewWarps * 2 * 256 * 32);
-    const long long fill = a.accumulate ? 0 : (t.rows + fill_rows - 1) / fill_rows;
+    // two CTAs an SM for the zeros, more where the bit map would not hold a CTA's rows
+    const long long share = (t.rows + 2 * num_sms() - 1) / (2 * num_sms()), zero_rows = share < kFewWarps * 2 * 256 * 32 ? share : kFewWarps * 2 * 256 * 32;
+    const long long fill = a.accumulate ? 0 : (t.rows + zero_rows - 1) / zero_rows;
     launch_pdl(embedding_few_kernel<T, VEC>, dim3(static_cast<unsigned>(a.blocks + fill)), dim3(kFewWarps * 32), 0, s, 1, t, a, vec_fill,
-               fill_rows);
+               static_cast<int>(zero_rows));
     return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
   }
   const int bits = key_bits(t.rows);
   SortBuffers b;
-  for (int k = 0; k < 2; ++k) {
-    b.key[k] = ws + 2ll * k * t.n;
-    b.pos[k] = ws + (2ll * k + 1) * t.n;
-  }
+  for (int k = 0; k < 2; ++k) b.at[k] = reinterpret_cast<Token*>(ws + 2ll * k * t.n);
   b.passes = (bits + 8) / 9;
   b.bits = (bits + b.passes - 1) / b.passes;
-  a.part = reinterpret_cast<float*>(ws + 4ll * t.n);
-  static unsigned long long ready = 0;      // per device
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= 64 || !(ready >> dev & 1)) {
-    if (cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortSmem) != cudaSuccess)
-      return kErrLaunch;
-    if (dev < 64) ready |= 1ull << dev;
-  }
-  // one CTA of the sort kernel an SM, in clusters of 8
-  const int fill_rows = fill_rows_of(t.rows, (num_sms() / kSortCtas - 1) * kSortCtas, static_cast<int>(kSortSmem) * 8);
-  const long long fill = a.accumulate ? 0 : (t.rows + fill_rows - 1) / fill_rows;
-  launch_pdl(embedding_sort_kernel, dim3(static_cast<unsigned>((1 + (fill + kSortCtas - 1) / kSortCtas) * kSortCtas)), dim3(kSortThreads),
-             kSortSmem, s, kSortCtas, t, b, a.dw, a.ldw, a.H, vec_fill, fill_rows);
-  const uint32_t* key = b.key[(b.passes - 1) & 1];
-  const uint32_t* pos = b.pos[(b.passes - 1) & 1];
+  uint32_t* seen = ws + 4ll * t.n;
+  a.part = reinterpret_cast<float*>(seen + (a.accumulate ? 0 : t.rows));
+  const int sort_ctas = sort_cluster(t.n);
+  if (!sort_ctas) return kErrLaunch;
+  if (!a.accumulate) launch_pdl(embedding_mark_kernel, dim3((t.n + 255) / 256), dim3(256), 0, s, 1, t, seen);
+  launch_pdl(embedding_sort_kernel, dim3(sort_ctas), dim3(kSortThreads), kSortSmem, s, sort_ctas, t, b);
+  const Token* tokens = b.at[(b.passes - 1) & 1];
   const int piece = sum_piece(t.n, a.H), length = piece * kSumWarps, chunks = (t.n + length - 1) / length;
-  const long long grid = static_cast<long long>(chunks) * a.blocks;
-  if (grid > 0x7fffffffll) return kErrTooLarge;
-  launch_pdl(embedding_sums_kernel<T, VEC>, dim3(static_cast<unsigned>(grid)), dim3(kSumWarps * 32), 0, s, 1, key, pos, t.n, piece, a);
-  launch_pdl(embedding_join_kernel<T, VEC>, dim3(static_cast<unsigned>((grid + 7) / 8)), dim3(256), 0, s, 1, key, t.n, length, chunks, a);
+  const long long items = static_cast<long long>(chunks) * a.blocks, fill = a.accumulate ? 0 : (t.rows + kZeroRows - 1) / kZeroRows;
+  if (items + fill > 0x7fffffffll) return kErrTooLarge;
+  if (!launch_beside(embedding_table_kernel<T, VEC>, static_cast<unsigned>(items + fill), kSumWarps * 32, s, t, tokens, seen, piece,
+                     static_cast<int>(fill), vec_fill, a))
+    return kErrLaunch;
+  launch_pdl(embedding_join_kernel<T, VEC>, dim3(static_cast<unsigned>((items + 15) / 16)), dim3(512), 0, s, 1, tokens, t.n, length, chunks, a);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
 }  // namespace tp
@@ -554,9 +620,9 @@ extern "C" int tp_embedding_fwd(int dtype, const void* ids, int ids64, int n, in
 
 // Workspace of tp_embedding_bwd in blocks of 256 bytes (base address: a multiple of 16).
 extern "C" int tp_embedding_bwd_workspace_blocks(int n, long long rows, int H) {
-  if (n <= kFewTokens) return 1;
+  if (n <= kFewTokens) return 0;
   const long long length = sum_piece(n, H) * kSumWarps, chunks = (n + length - 1) / length, blocks = (H + 255) / 256;
-  const long long bytes = 16ll * n + chunks * 2 * blocks * 256 * 4;
+  const long long bytes = 16ll * n + 4 * rows + chunks * 2 * blocks * 256 * 4;
   return static_cast<int>((bytes + 255) / 256);
 }
 

@@ -39,13 +39,33 @@ template <typename T> struct Granule {
   }
 };
 
+// i / d for 0 <= i < 2^31 as a multiplication: with 2^(l-1) < d <= 2^l, m = floor(2^(31+l) / d) + 1 has 32 bits and
+// (i m) >> (31 + l) is the quotient, as m d exceeds 2^(31+l) by at most d <= 2^l.
+struct Divider {
+  uint32_t d, mul;
+  int shift;
+  Divider() = default;
+  __host__ explicit Divider(int d_) : d(d_), mul(0), shift(0) {
+    if (d > 1) {
+      int l = 1;
+      while ((1ull << l) < d) ++l;
+      mul = static_cast<uint32_t>((1ull << (31 + l)) / d + 1);
+      shift = l - 1;
+    }
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t i) const { return d == 1 ? i : __umulhi(i, mul) >> shift; }
+};
+
 // Element offset of outer index i of an array [*, cols] of rows with strides s0 and s1: a batch-first array read in
 // sequence-first order needs no copy.
 struct OuterIndex {
   long long s0, s1;
-  int cols;
+  Divider cols;
+  OuterIndex() = default;
+  __host__ OuterIndex(long long s0_, long long s1_, int cols_) : s0(s0_), s1(s1_), cols(cols_) {}
   __device__ __forceinline__ long long operator()(int i) const {
-    return cols == 1 ? i * s0 : (i / cols) * s0 + (i % cols) * s1;
+    const uint32_t q = cols(i);
+    return q * s0 + (i - q * cols.d) * s1;
   }
 };
 

@@ -363,7 +363,7 @@ def embedding_fwd(ids, weight, out=None, *, scale: float = 1.0, first_row: int =
 
 
 def embedding_bwd_workspace_bytes(n: int, rows: int, H: int) -> int:
-    return cuda_lib().tp_embedding_bwd_workspace_blocks(int(n), int(rows), int(H)) * 256
+    return max(1, cuda_lib().tp_embedding_bwd_workspace_blocks(int(n), int(rows), int(H))) * 256
 
 
 def embedding_bwd(ids, dy, dweight, *, scale: float = 1.0, first_row: int = 0, padding_id: Optional[int] = None,
@@ -385,15 +385,16 @@ def embedding_bwd(ids, dy, dweight, *, scale: float = 1.0, first_row: int = 0, p
     lib = cuda_lib()
     blocks = lib.tp_embedding_bwd_workspace_blocks(n, rows, H)
     if workspace is None:
-        workspace = torch.empty(blocks * 256, dtype=torch.uint8, device=dweight.device)
-    elif workspace.numel() * workspace.element_size() < blocks * 256 or not workspace.is_contiguous() \
+        if blocks:      # (few tokens need none)
+            workspace = torch.empty(blocks * 256, dtype=torch.uint8, device=dweight.device)
+    elif workspace.numel() * workspace.element_size() < max(blocks, 1) * 256 or not workspace.is_contiguous() \
             or workspace.data_ptr() % 16:
-        raise KernelError(f"workspace of {blocks * 256} contiguous bytes on a 16-byte boundary")
+        raise KernelError(f"workspace of {max(blocks, 1) * 256} contiguous bytes on a 16-byte boundary")
     _same_device(ids, dy, dweight, workspace)
     cols, s0, s1 = _outer(ids, 0, n, "ids")
     st = lib.tp_embedding_bwd(_kind(dy, _DT_ROWS, "dy"), ids.data_ptr(), _kind(ids, _DT_IDS, "ids"), n, cols, s0, s1,
                               first_row, -1 if padding_id is None else padding_id, dy.data_ptr(), ldy, dweight.data_ptr(),
-                              ldw, rows, H, scale, int(accumulate), workspace.data_ptr(), _stream())
+                              ldw, rows, H, scale, int(accumulate), _ptr(workspace), _stream())
     if st:
         check(st, "tp_embedding_bwd")
     return dweight
