@@ -287,38 +287,45 @@ template <int LEFT> __device__ __forceinline__ void cp_async_wait() {
 }
 
 // ------------------------------------------------------------------ rows held on chip
-// Logits are read once and, with WRITE, their gradient is written: what bounds the kernel is those bytes.  A row belongs to a
-// cluster of 1 to 8 CTAs of THREADS threads, NG granules a thread.  The next row travels into shared memory (cp.async, slots that
-// only their thread reads) while this one is worked on; its exponentials, relative to the thread's own largest logit, stay in
-// registers in fp32 until the row's sum is known, so each is computed once: two a logit and softmax would
-// keep the exponential unit (16 a cycle and SM) busy three quarters of the time that the bytes take, and two softmaxes of
-// different temperature (DUAL) longer than that.  Without DUAL there is one exponential a logit: the temperature
-// is 1 or one of the two terms has no weight.
+// Logits are read once and, with WRITE, their gradient is written: what bounds the kernel is those bytes, next to it the
+// instructions of a row.  A row belongs to a cluster of 1 to 8 CTAs, each with THREADS threads that hold NG granules and one warp
+// that does everything a row needs once.  That warp has the next two rows copied into shared memory (cp.async.bulk); the others'
+// exponentials, relative to the thread's own largest logit, stay in registers in fp32 until the row's sum is known, so each is
+// computed once: two a logit and softmax would keep the exponential unit (16 a cycle and SM) busy three quarters of the time that
+// the bytes take, and two softmaxes of different temperature (DUAL) longer than that.  Without DUAL there is one
+// exponential a logit: the temperature is 1 or one of the two terms has no weight.
 //
-// Warps do not meet at barriers for the sums: each sends its own to every CTA of the cluster (st.async, counted by an mbarrier)
-// and adds up all of them, so that fast warps run ahead into the next row.
-//
-// The teacher's entries: thread k of every CTA has entry k, and stores its element of the gradient again after the row's where
-// it lies in the CTA's part.  A small hash table of their ids tells whether one occurs twice: only then are all entries
-// looked through for their sum.
+// There are no barriers of the CTA.  Per row, with two of each in turn: `full` (the row is in shared memory), `parts_in` (the
+// sums of all warps of the cluster have arrived, by st.async where it has several CTAs), `known` (the extra warp has added them
+// up), `written` (the CTA's part of the gradient is stored).  The label's and the teacher's elements of the gradient are then
+// stored again by the extra warp, while the others are on the next row.
+constexpr int kRowsAhead = 2;
 
 // CTAs an SM has registers for, by the exponentials a thread keeps.
-constexpr int loss_ctas_per_sm(int threads, int values) { return (values > 32 ? 512 : values > 16 ? 768 : 1024) / threads; }
+constexpr int loss_ctas_per_sm(int threads, int values) {
+  const int regs = values > 32 ? 112 : values > 16 ? 72 : 56, n = 65536 / (regs * (threads + 32));
+  return n < 1 ? 1 : n > 8 ? 8 : n;
+}
 
-// What a warp knows of its part of a row.
+// What a warp knows of its part of a row: its largest logit, sums of exponentials relative to that (to 0 where it is -inf).
 struct alignas(16) WarpPart {
-  float m, s1;            // largest logit; sum of exponentials relative to it (to 0 where it is -inf)
-  float zy, own;          // z_y - m and 1 where the label is in the warp's part
-  float t_max, t_sum;     // over the warp's entries: largest t, sum of exp((t - t_max) / T)
-  float entropy, st;      // the same weighted with (t - t_max) / T; the second softmax's sum
-  float dot, mass;        // over its entries in this CTA's part, as t_sum: p (z - m), p
-  float pad[2];
+  float m, s1, st, pad;
 };
-// Stores a part into a CTA's shared memory; its bytes count on that CTA's barrier.  (A cluster barrier would do as
+// What all need of a whole row.
+struct alignas(16) RowKnown {
+  float m, c1, ct;     // largest logit; factors of exponentials relative to it
+  int active;          // 0: the gradient is zero
+};
+
+// Stores 16 bytes into a CTA's shared memory; they count on that CTA's barrier.  (A cluster barrier would do as
 // well, but its release waits for all of the CTA's stores to global memory, a row's gradient each time.)
-__device__ __forceinline__ void send16(uint32_t cluster_addr, uint32_t cluster_bar, float a, float b, float c, float d) {
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];"
-               ::"r"(cluster_addr), "f"(a), "f"(b), "f"(c), "f"(d), "r"(cluster_bar) : "memory");
+__device__ __forceinline__ void send16(uint32_t cluster_addr, uint32_t cluster_bar, float a, float b, float c) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %3}, [%4];"
+               ::"r"(cluster_addr), "f"(a), "f"(b), "f"(c), "r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 
 constexpr int loss_table_size(int top) {      // slots of the hash table: a power of two, at least twice the entries
@@ -327,313 +334,338 @@ constexpr int loss_table_size(int top) {      // slots of the hash table: a powe
   return n;
 }
 
+// Granules of a row in the part that begins with granule g0: their number, and those of its first and last where others'
+// elements lie in them (numbers in the part, or -1; a granule that is both is the first).
+struct PartGeom {
+  int count, first, last;
+  template <typename T> __device__ __forceinline__ PartGeom(const RowPieces<T>& r, int g0, int per) {
+    constexpr int N = Granule<T>::N;
+    count = min(r.count - g0, per);
+    first = g0 == 0 && r.lead > 0 && count > 0 ? 0 : -1;
+    const int end = r.count - 1 - g0;
+    last = (r.lead + r.V) % N != 0 && end >= 0 && end < count ? end : -1;
+    if (last == first) last = -1;
+  }
+};
+
 template <typename T, bool DUAL, int THREADS, int NG, bool WRITE>
-__global__ void __launch_bounds__(THREADS, loss_ctas_per_sm(THREADS, (WRITE ? NG : 1) * Granule<T>::N * (DUAL ? 2 : 1)))
+__global__ void __launch_bounds__(THREADS + 32, loss_ctas_per_sm(THREADS, (WRITE ? NG : 1) * Granule<T>::N * (DUAL ? 2 : 1)))
 loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
-  constexpr int N = Granule<T>::N, kWarps = THREADS / 32, kSlots = THREADS * NG, kKept = WRITE ? NG : 1, kMaxParts = 8;
+  constexpr int N = Granule<T>::N, kWarps = THREADS / 32, kSlots = THREADS * NG, kKept = WRITE ? NG : 1, kMaxParts = 8, kAhead = 4;
   extern __shared__ __align__(16) uint4 loss_smem[];
-  uint4* raw = loss_smem;                                      // [2][kSlots]
-  float* top_p = reinterpret_cast<float*>(raw + 2 * kSlots);   // [top] exp((t - its warp's t_max) / T), then relative to the row's
-  float* top_z = top_p + a.top;                                // [top] z
-  int* top_id = reinterpret_cast<int*>(top_z + a.top);         // [top]
-  int* ids = top_id + a.top;                                   // [2][table] hash tables of id + 1
-  __shared__ WarpPart inbox[2][kMaxParts * kWarps];
-  __shared__ uint64_t arrived[2];      // all parts of a row are in inbox[.]
-  __shared__ int twice[2], abort_word;
+  uint4* raw = loss_smem;                                          // [2][kSlots]
+  float* top_p_all = reinterpret_cast<float*>(raw + 2 * kSlots);   // [2][top] first t, then exp((t - t_max) / T)
+  float* top_z_all = top_p_all + 2 * a.top;                        // [2][top] z, where it is needed
+  int* top_id_all = reinterpret_cast<int*>(top_z_all + 2 * a.top); // [2][top]
+  int* ids = top_id_all + 2 * a.top;                               // [table] hash table of id + 1
+  __shared__ WarpPart inbox[2][kMaxParts * kWarps + 1];
+  __shared__ RowKnown known_row[2];
+  __shared__ uint64_t full[2], parts_in[2], known[2], written[2];
+  __shared__ int abort_word;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = parts > 1 ? cluster_ctarank() : 0;
-  const int stride = gridDim.x / parts, g0 = rank * per, warps = parts * kWarps;
+  const int stride = gridDim.x / parts, g0 = rank * per, senders = parts * kWarps;
   const float inv_t = 1.0f / a.temperature, kt = inv_t * kLog2e;
   // the one exponential's exponent without DUAL: z, or with a teacher alone z / T
   const float k1 = DUAL || a.weight == 0.0f ? kLog2e : kt;
-  const T* z0 = static_cast<const T*>(a.logits);
-  const bool teacher = a.top > 0, full = DUAL || teacher;      // full: all of a WarpPart travels, else its first 16 bytes
   const WaitCtx wait{&abort_word, a.status};
   if (tid == 0) {
     abort_word = 0;
-    twice[0] = twice[1] = 0;
-    // (a launch without clusters has no st.async: its warps store their parts and arrive)
-    mbar_init(&arrived[0], parts > 1 ? 1 : kWarps);
-    mbar_init(&arrived[1], parts > 1 ? 1 : kWarps);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&parts_in[i], parts > 1 ? 1 : kWarps + 1);      // (a launch without clusters has no st.async)
+      mbar_init(&known[i], 1);
+      mbar_init(&written[i], kWarps);
+    }
     fence_barrier_init();
   }
-  for (int i = tid; i < 2 * table; i += THREADS) ids[i] = 0;
   if (parts > 1) cluster_sync_all();
   else __syncthreads();
   pdl_wait();
 
-  const uint32_t raw_addr = smem_u32(raw + tid);
-  // Granules k < kFull are there for every thread, and none of them is a row's last (see loss_rows_fit): a test for each
-  // granule costs half as much as the work on it.
-  constexpr int kFull = NG > 2 ? NG - 2 : 0;
-  auto prefetch = [&](const T* z, int buf) {
-    const RowPieces<T> r(z, a.V);
-    const int cnt = min(r.count - g0, per);
-    const T* src = z + ((g0 + tid) * N - r.lead);
-    const uint32_t dst = raw_addr + buf * (kSlots * 16);
-    const int left = (r.lead + r.V - (g0 + tid) * N) * static_cast<int>(sizeof(T));
-#pragma unroll
-    for (int k = 0; k < NG; ++k) {
-      // (the first granule may begin in the row before, but not before the matrix)
-      if (k == 0 ? tid < cnt && src >= z0 : k < kFull || tid + k * THREADS < cnt)
-        cp_async_16(dst + k * THREADS * 16, src + k * THREADS * N, k < kFull ? 16 : min(left - k * THREADS * 16, 16));
-    }
-  };
-
-  int row = blockIdx.x / parts, buf = 0, turn = 0;
-  const T* z = z0 + row * a.ld;
-  T* out = static_cast<T*>(a.dlogits) + row * a.ldd;
+  const int row0 = blockIdx.x / parts;
+  const T* z = static_cast<const T*>(a.logits) + row0 * a.ld;
+  T* out = static_cast<T*>(a.dlogits) + row0 * a.ldd;
   const long long z_step = stride * a.ld, out_step = stride * a.ldd;
-  RawLabel label_next{};
-  RawEntry entry_next{-1, 0};
-  float g_next = 1.0f;
-  if (row < a.rows) {
-    prefetch(z, 0);
-    label_next.load(a, row);
-    if (tid < a.top) entry_next.load(a, row, tid);
-    if (WRITE && a.grad_loss) g_next = a.grad_loss[row * a.ldg];
-  }
-  cp_async_commit();
-  for (; row < a.rows; row += stride, z += z_step, out += out_step, buf ^= 1, turn += buf == 0) {
-    const int label = label_next.get(a);
-    const RawEntry entry = entry_next;
-    const float g = g_next;
-    if (row + stride < a.rows) {
-      prefetch(z + z_step, buf ^ 1);
-      label_next.load(a, row + stride);
-      if (tid < a.top) entry_next.load(a, row + stride, tid);
-      if (WRITE && a.grad_loss) g_next = a.grad_loss[(row + stride) * a.ldg];
-    }
-    cp_async_commit();
-    const RowPieces<T> r(z, a.V);
-    uint4* mine = raw + buf * kSlots + tid;
-    const int cnt = min(r.count - g0, per);
-    auto place = [&](int id) {      // number in this part of an element's granule, -1 in another part
-      const int gl = static_cast<int>(static_cast<unsigned>(id + r.lead) / N) - g0;
-      return id >= 0 && gl >= 0 && gl < per ? gl : -1;
-    };
-    // entry tid's logit is on its way while the row is worked on
-    float z_entry = 0.0f;
-    if (tid < a.top && place(entry.id(a)) >= 0) z_entry = Elem<T>::to_f(z[entry.id(a)]);
-    cp_async_wait<1>();
-    // the row's first and last granule, where others' elements lie in them: numbers in this part, or -1
-    const int first = g0 == 0 && r.lead > 0 && cnt > 0 ? 0 : -1;
-    const int last = (r.lead + r.V) % N != 0 && r.count - 1 - g0 < cnt ? r.count - 1 - g0 : -1;
-    const bool owns_first = first == 0 && tid == 0, owns_last = last >= 0 && last != first && tid == (last & (THREADS - 1));
-    if (owns_first) mine[0] = z - r.lead >= z0 ? r.mask_edge(mine[0], 0) : r.load_edge(0);
-    if (owns_last) mine[last - tid] = r.mask_edge(mine[last - tid], g0 + last);
-    // ---- the thread's largest logit and exponentials
-    GranuleMax<T> largest;
+
+  if (warp < kWarps) {
+    // ================================================================ the row's logits
+    constexpr int kFull = NG > 2 ? NG - 2 : 0;      // granules that every thread has (see loss_rows_fit)
+    for (int row = row0, buf = 0, turn = 0; row < a.rows; row += stride, z += z_step, out += out_step, buf ^= 1, turn ^= buf == 0) {
+      const RowPieces<T> r(z, a.V);
+      const PartGeom geom(r, g0, per);
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[buf], turn, wait, kErrWaitProducer))) break;
+      const uint4* mine = raw + buf * kSlots + tid;
+      GranuleMax<T> largest;
 #pragma unroll
-    for (int k = 0; k < NG; ++k)
-      if (k < kFull || tid + k * THREADS < cnt) largest.add(mine[k * THREADS]);
-    const float m_own = largest.get(), shift = m_own == -INFINITY ? 0.0f : m_own;
-    const Exponent x1{k1, shift}, xt{kt, shift};
-    float e1[kKept][N], et[DUAL ? kKept : 1][N], s1 = 0.0f, st = 0.0f;
+      for (int k = 0; k < NG; ++k)
+        if (k < kFull || tid + k * THREADS < geom.count) largest.add(mine[k * THREADS]);
+      const float m_own = largest.get(), shift = m_own == -INFINITY ? 0.0f : m_own;
+      const Exponent x1{k1, shift}, xt{kt, shift};
+      float e1[kKept][N], et[DUAL ? kKept : 1][N], s1 = 0.0f, st = 0.0f;
 #pragma unroll
-    for (int k = 0; k < NG; ++k) {
-      const int kept = WRITE ? k : 0;
-      if (k >= kFull && tid + k * THREADS >= cnt) continue;
-      const uint4 u = mine[k * THREADS];
-      granule_exp<T>(u, x1, e1[kept]);
-      s1 += sum_of<N>(e1[kept]);
-      if (DUAL) {
-        granule_exp<T>(u, xt, et[kept]);
-        st += sum_of<N>(et[kept]);
-      }
-    }
-    // ---- the warp's
-    const float m_warp = warp_max(m_own), m_from = m_warp == -INFINITY ? 0.0f : m_warp;
-    s1 = warp_add(s1 * Exponent{k1, m_from}.factor(m_own));
-    if (DUAL) st = warp_add(st * Exponent{kt, m_from}.factor(m_own));
-    const int label_gl = place(label);
-    const bool owner = label_gl >= 0 && tid == (label_gl & (THREADS - 1));      // of the label's granule
-    float zy = 0.0f;
-    if (owner) zy = Elem<T>::to_f(reinterpret_cast<const T*>(mine + (label_gl - tid))[static_cast<unsigned>(label + r.lead) % N]);
-    const unsigned label_lane = __ballot_sync(0xffffffffu, owner);
-    const float zy_warp = __shfl_sync(0xffffffffu, zy, label_lane ? __ffs(label_lane) - 1 : 0);
-    float t_max = -INFINITY, t_sum = 0.0f, entropy = 0.0f, dot = 0.0f, mass = 0.0f;
-    if (teacher) {
-      for (int k = tid; k < a.top; k += THREADS) {
-        RawEntry e = entry;
-        float v = z_entry;
-        if (k >= THREADS) {
-          e.load(a, row, k);
-          v = place(e.id(a)) >= 0 ? Elem<T>::to_f(z[e.id(a)]) : 0.0f;
+      for (int k = 0; k < NG; ++k) {
+        const int kept = WRITE ? k : 0;
+        if (k >= kFull && tid + k * THREADS >= geom.count) continue;
+        const uint4 u = mine[k * THREADS];
+        granule_exp<T>(u, x1, e1[kept]);
+        s1 += sum_of<N>(e1[kept]);
+        if (DUAL) {
+          granule_exp<T>(u, xt, et[kept]);
+          st += sum_of<N>(et[kept]);
         }
-        const int id = e.id(a);
-        top_id[k] = id;
-        top_p[k] = e.logit(a);
-        top_z[k] = v;
-        t_max = fmaxf(t_max, top_p[k]);
-        if (WRITE && place(id) >= 0) {
-          int slot = (id * 0x9e3779b1u) >> 20 & (table - 1);
-          while (true) {      // (at most half of the slots are ever taken)
-            const int was = atomicCAS(&ids[buf * table + slot], 0, id + 1);
-            if (was == 0) break;
-            if (was == id + 1) {
-              twice[buf] = 1;
-              break;
-            }
-            slot = (slot + 1) & (table - 1);
+      }
+      const float m_warp = warp_max(m_own), m_from = m_warp == -INFINITY ? 0.0f : m_warp;
+      s1 = warp_add(s1 * Exponent{k1, m_from}.factor(m_own));
+      if (DUAL) st = warp_add(st * Exponent{kt, m_from}.factor(m_own));
+      // (without a gradient to wait for: whoever has all sums of a row knows that those of the row before have been read)
+      if (!WRITE && row != row0 &&
+          !__all_sync(0xffffffffu, mbar_wait(&known[buf ^ 1], buf ? turn : turn ^ 1, wait, kErrWaitPeer))) break;
+      if (parts > 1) {
+        if (lane < parts)
+          send16(mapa_u32(smem_u32(&inbox[buf][rank * kWarps + warp]), lane), mapa_u32(smem_u32(&parts_in[buf]), lane), m_warp, s1, st);
+      } else if (lane == 0) {
+        inbox[buf][warp] = WarpPart{m_warp, s1, st, 0.0f};
+        mbar_arrive(&parts_in[buf]);
+      }
+      if (!WRITE) continue;
+      if (!__all_sync(0xffffffffu, mbar_wait(&known[buf], turn, wait, kErrWaitPeer))) break;
+      const RowKnown w = known_row[buf];
+      const bool wide = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(z)) & 15) == 0;
+      if (!w.active) {
+        const float o[N] = {};
+        for (int gl = tid; gl < geom.count; gl += THREADS) r.store(out, g0 + gl, o, wide && gl != geom.first && gl != geom.last);
+      } else {
+        const float c1 = w.c1 * Exponent{k1, w.m}.factor(m_own), ct = DUAL ? w.ct * Exponent{kt, w.m}.factor(m_own) : 0.0f;
+        T* o = out + ((g0 + tid) * N - r.lead);
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+          const int gl = tid + k * THREADS;
+          if (k >= kFull && gl >= geom.count) continue;
+          float v[N];
+#pragma unroll
+          for (int j = 0; j < N; j += 2) {
+            float2 d = mul2(make_float2(e1[k][j], e1[k][j + 1]), dup2(c1));
+            if (DUAL) d = fma2(make_float2(et[k][j], et[k][j + 1]), dup2(ct), d);
+            v[j] = d.x;
+            v[j + 1] = d.y;
           }
+          if (wide && !(k == 0 && gl == geom.first) && !(k >= kFull && gl == geom.last))
+            *reinterpret_cast<uint4*>(o + k * THREADS * N) = Granule<T>::pack(v);
+          else
+            r.store(out, g0 + gl, v, false);
         }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&written[buf]);
+    }
+  } else {
+    // ================================================================ what a row needs once
+    auto in_part = [&](const RowPieces<T>& r, int id) {
+      const int gl = static_cast<int>(static_cast<unsigned>(id + r.lead) / N) - g0;
+      return id >= 0 && gl >= 0 && gl < per;
+    };
+    // lanes 0 .. N - 1 have the first granule's elements, lanes 16 .. the last's, where these are not all the row's
+    auto load_edge = [&](const T* z) {
+      const RowPieces<T> r(z, a.V);
+      const PartGeom geom(r, g0, per);
+      const int gl = lane < 16 ? geom.first : geom.last, i = (g0 + gl) * N - r.lead + (lane & 15);
+      return gl >= 0 && (lane & 15) < N && i >= 0 && i < a.V ? z[i] : Elem<T>::from_f(-INFINITY);
+    };
+    int fetched[2] = {0, 0};      // rows that each of the two places has been given
+    auto fetch = [&](const T* z, int buf, T edge) {
+      if (buf) ++fetched[1];
+      else ++fetched[0];
+      const RowPieces<T> r(z, a.V);
+      const PartGeom geom(r, g0, per);
+      const int gl = lane < 16 ? geom.first : geom.last;
+      if (gl >= 0 && (lane & 15) < N) reinterpret_cast<T*>(raw + buf * kSlots + gl)[lane & 15] = edge;
+      __syncwarp();
+      if (lane == 0) {
+        const int from = geom.first == 0 ? 1 : 0, to = geom.last >= 0 ? geom.last : geom.count;
+        const uint32_t bytes = to > from ? (to - from) * 16u : 0u;
+        mbar_expect_tx(&full[buf], bytes);
+        if (bytes) bulk_load(smem_u32(raw + buf * kSlots + from), z + ((g0 + from) * N - r.lead), bytes, &full[buf]);
+      }
+    };
+    // the label and the first kAhead * 32 entries of a row as they come
+    RawLabel raw_label{};
+    RawEntry raw_entry[kAhead];
+    float raw_g = 1.0f;
+    auto load_raw = [&](int row) {
+      raw_label.load(a, row);
+      if (WRITE && a.grad_loss) raw_g = a.grad_loss[row * a.ldg];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (lane + 32 * j < a.top) raw_entry[j].load(a, row, lane + 32 * j);
+    };
+    // ... and of the next row as they are needed: the entries, with t_sum and whether an id occurs twice, are in half `half` of
+    // the arrays.  rank 0 has all logits, for the loss, the others those of their part.
+    int label = -1;
+    float zy = 0.0f, g = 1.0f, t_sum = 0.0f, entropy = 0.0f, z_entry[kAhead];
+    bool twice = false;
+    auto wants = [&](const RowPieces<T>& r, int id) { return id >= 0 && (rank == 0 || in_part(r, id)); };
+    auto begin_entries = [&](const T* z, int row, int half) {
+      const RowPieces<T> r(z, a.V);
+      label = raw_label.get(a);
+      g = raw_g;
+      zy = wants(r, label) ? Elem<T>::to_f(z[label]) : 0.0f;
+      for (int k0 = 0; k0 < a.top; k0 += 32 * kAhead) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          const int k = k0 + lane + 32 * j;
+          if (k >= a.top) continue;
+          RawEntry e = raw_entry[j];
+          if (k0 > 0) e.load(a, row, k);
+          const int id = e.id(a);
+          top_id_all[half * a.top + k] = id;
+          top_p_all[half * a.top + k] = e.logit(a);
+          const float v = wants(r, id) ? Elem<T>::to_f(z[id]) : 0.0f;
+          if (k0 == 0) z_entry[j] = v;
+          else top_z_all[half * a.top + k] = v;
+        }
+      }
+    };
+    auto end_entries = [&](const T* z, int half) {
+      const RowPieces<T> r(z, a.V);
+      float* top_p = top_p_all + half * a.top;
+      int* top_id = top_id_all + half * a.top;
+      float t_max = -INFINITY;
+      t_sum = entropy = 0.0f;
+      twice = false;
+      if (a.top == 0) return;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (lane + 32 * j < a.top) top_z_all[half * a.top + lane + 32 * j] = z_entry[j];
+      for (int k = lane; k < a.top; k += 32) t_max = fmaxf(t_max, top_p[k]);
       t_max = warp_max(t_max);
-      const float t_from = t_max == -INFINITY ? 0.0f : t_max;
-      for (int k = tid; k < a.top; k += THREADS) {
-        const float lt = (top_p[k] - t_from) * inv_t, p = top_id[k] >= 0 ? exp2_approx(lt * kLog2e) : 0.0f;
+      if (t_max == -INFINITY) t_max = 0.0f;
+      for (int k = lane; k < a.top; k += 32) {
+        const float lt = (top_p[k] - t_max) * inv_t, p = top_id[k] >= 0 ? exp2_approx(lt * kLog2e) : 0.0f;
         top_p[k] = p;
         t_sum += p;
-        if (p == 0.0f) continue;
-        entropy += p * lt;
-        if (place(top_id[k]) < 0) continue;
-        dot += p * (top_z[k] - m_from);
-        mass += p;
+        if (p != 0.0f) entropy += p * lt;
       }
       t_sum = warp_add(t_sum);
       entropy = warp_add(entropy);
-      dot = warp_add(dot);
-      mass = warp_add(mass);
-    }
-    // ---- to all CTAs of the cluster, and all of it back
-    zy = label_lane ? zy_warp - m_from : 0.0f;
-    const float own = label_lane ? 1.0f : 0.0f;
-    if (parts > 1) {
-      if (tid == 0) mbar_expect_tx(&arrived[buf], warps * (full ? 48 : 16));
-      if (lane < parts) {
-        const uint32_t to = mapa_u32(smem_u32(&inbox[buf][rank * kWarps + warp]), lane), bar = mapa_u32(smem_u32(&arrived[buf]), lane);
-        send16(to, bar, m_warp, s1, zy, own);
-        if (full) {
-          send16(to + 16, bar, t_max, t_sum, entropy, st);
-          send16(to + 32, bar, dot, mass, 0.0f, 0.0f);
-        }
-      }
-    } else if (lane == 0) {
-      inbox[buf][warp] = WarpPart{m_warp, s1, zy, own, t_max, t_sum, entropy, st, dot, mass, {0.0f, 0.0f}};
-      mbar_arrive(&arrived[buf]);
-    }
-    bool ok = mbar_wait(&arrived[buf], turn & 1, wait, kErrWaitPeer);
-    float m = -INFINITY;
-    for (int i = lane; i < warps; i += 32) m = fmaxf(m, inbox[buf][i].m);
-    m = warp_max(m);
-    if (m == -INFINITY) m = 0.0f;
-    s1 = st = 0.0f;
-    for (int i = lane; i < warps; i += 32) {
-      s1 += inbox[buf][i].s1 * Exponent{k1, m}.factor(inbox[buf][i].m);
-      if (DUAL) st += inbox[buf][i].st * Exponent{kt, m}.factor(inbox[buf][i].m);
-    }
-    s1 = warp_add(s1);
-    st = DUAL ? warp_add(st) : s1;
-    const float my_t = t_max;
-    if (teacher) {      // (every CTA has all entries: its own warps' sums are enough)
-      const WarpPart& p = inbox[buf][rank * kWarps + (lane & (kWarps - 1))];
-      t_max = warp_max(p.t_max);
-      if (t_max == -INFINITY) t_max = 0.0f;
-      t_sum = warp_add<kWarps>(p.t_max == -INFINITY ? 0.0f : p.t_sum * exp2_approx((p.t_max - t_max) * kt));
-    }
-    const bool teach = a.weight != 0.0f && t_sum != 0.0f, zero = !(teach || label >= 0) || s1 == 0.0f;
-    if (rank == 0 && warp == 0) {
-      zy = entropy = dot = 0.0f;
-      for (int i = lane; i < warps; i += 32) {
-        const WarpPart& p = inbox[buf][i];
-        const float from = p.m == -INFINITY ? 0.0f : p.m;
-        zy += p.zy + p.own * (from - m);
-        if (teacher && p.t_max != -INFINITY) {
-          const float ft = (p.t_max - t_max) * inv_t, scale = exp2_approx(ft * kLog2e);
-          if (scale != 0.0f) {
-            dot += scale * (p.dot + p.mass * (from - m));
-            if (i < kWarps) entropy += scale * (p.entropy + p.t_sum * ft);
-          }
-        }
-      }
-      zy = warp_add(zy);
-      if (teacher) {
-        dot = warp_add(dot);
-        entropy = warp_add(entropy);
-      }
-      if (lane == 0) store_loss(a, row, WholeRow{m, s1, st, dot, zy}, label >= 0, teach, t_sum, entropy);
-    }
-    if (WRITE) {
-      // ---- the gradient
-      const RowFactors f(a, g, label >= 0, teach);
-      const float c1 = (DUAL ? f.g1 : f.g1 + f.gt) * (1.0f / s1) * Exponent{k1, m}.factor(m_own);
-      const float ct = DUAL ? f.gt * (1.0f / st) * Exponent{kt, m}.factor(m_own) : 0.0f;
-      const bool wide = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(z)) & 15) == 0;
-      if (!ok) {
-        // (nothing is known of the row)
-      } else if (zero) {
-        const float o[N] = {};
-        for (int gl = tid; gl < cnt; gl += THREADS) r.store(out, g0 + gl, o, wide && gl != first && gl != last);
+      if (!WRITE) return;
+      if (a.top <= 32) {
+        const int id = lane < a.top ? top_id[lane] : -1;
+        const unsigned same = __match_any_sync(0xffffffffu, id);
+        twice = __any_sync(0xffffffffu, id >= 0 && (same & (same - 1)) != 0);
       } else {
-        auto value = [&](float v1, float vt) { return DUAL ? fmaf(ct, vt, c1 * v1) : c1 * v1; };
-        if (wide) {
-          uint4* o = reinterpret_cast<uint4*>(out + ((g0 + tid) * N - r.lead));
-#pragma unroll
-          for (int k = 0; k < NG; ++k) {
-            const int gl = tid + k * THREADS;
-            if ((k >= kFull && (gl >= cnt || gl == last)) || (k == 0 && gl == first)) continue;
-            float v[N];
-#pragma unroll
-            for (int j = 0; j < N; j += 2) {
-              float2 d = mul2(make_float2(e1[k][j], e1[k][j + 1]), dup2(c1));
-              if (DUAL) d = fma2(make_float2(et[k][j], et[k][j + 1]), dup2(ct), d);
-              v[j] = d.x;
-              v[j + 1] = d.y;
-            }
-            o[k * THREADS] = Granule<T>::pack(v);
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < NG; ++k) {
-            const int gl = tid + k * THREADS;
-            if (gl >= cnt || gl == first || gl == last) continue;
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-              out[(g0 + gl) * N - r.lead + j] = Elem<T>::from_f(value(e1[k][j], DUAL ? et[k][j] : 0.0f));
+        bool mine = false;
+        for (int i = lane; i < table; i += 32) ids[i] = 0;
+        __syncwarp();
+        for (int k = lane; k < a.top; k += 32) {
+          const int id = top_id[k];
+          if (!in_part(r, id)) continue;
+          int slot = static_cast<int>(id * 0x9e3779b1u >> 16) & (table - 1);
+          while (true) {      // (at most half of the slots are ever taken)
+            const int was = atomicCAS(&ids[slot], 0, id + 1);
+            mine |= was == id + 1;
+            if (was == 0 || was == id + 1) break;
+            slot = (slot + 1) & (table - 1);
           }
         }
-        if (owns_first || owns_last) {
-          for (int which = owns_first ? 0 : 1; which < (owns_last ? 2 : 1); ++which) {
-            const uint4 u = which ? mine[last - tid] : mine[0];
-            float v1[N], vt[N] = {};
-            granule_exp<T>(u, x1, v1);
-            if (DUAL) granule_exp<T>(u, xt, vt);
-#pragma unroll
-            for (int j = 0; j < N; ++j) v1[j] = value(v1[j], vt[j]);
-            r.store(out, which ? g0 + last : 0, v1, false);
-          }
-        }
-        if (owner) {      // over what this thread has just stored
-          const float v = Elem<T>::to_f(reinterpret_cast<const T*>(mine + (label_gl - tid))[static_cast<unsigned>(label + r.lead) % N]);
-          out[label] = Elem<T>::from_f((c1 * exp2_approx(x1(v)) - f.g1) + (DUAL ? ct * exp2_approx(xt(v)) : 0.0f));
-        }
+        twice = __any_sync(0xffffffffu, mine);
       }
-      if (teacher) {
-        const float scale = my_t == -INFINITY ? 0.0f : exp2_approx((my_t - t_max) * kt);
-        for (int k = tid; k < a.top; k += THREADS) top_p[k] *= scale;
-        ok = __syncthreads_and(ok);      // the row's stores come before the entries', and the table is complete
-        const bool look = twice[buf];
-        if (ok && teach && !zero) {
-          const Exponent y1{k1, m}, yt{kt, m};
-          const float r1 = (DUAL ? f.g1 : f.g1 + f.gt) * (1.0f / s1), rt = DUAL ? f.gt * (1.0f / st) : 0.0f;
-          for (int k = tid; k < a.top; k += THREADS) {
-            if (place(top_id[k]) >= 0)
-              store_entry<T, DUAL>(out, top_id[k], k, exp2_approx(y1(top_z[k])), DUAL ? exp2_approx(yt(top_z[k])) : 0.0f, top_id, top_p,
-                                   a.top, look, r1, rt, f.g1, f.gt / t_sum, label);
-          }
+    };
+    // rank 0 has what it needs of the row's logits: the gradient may take their place
+    auto announce = [&](int buf) {
+      __syncwarp();
+      if (parts > 1) {
+        if (lane == 0) mbar_expect_tx(&parts_in[buf], (senders + 1) * 16);
+        if (rank == 0 && lane < parts)
+          send16(mapa_u32(smem_u32(&inbox[buf][senders]), lane), mapa_u32(smem_u32(&parts_in[buf]), lane), zy, 0.0f, 0.0f);
+      } else if (lane == 0) {
+        mbar_arrive(&parts_in[buf]);
+      }
+    };
+
+    T edge = Elem<T>::from_f(-INFINITY);
+    if (row0 < a.rows) {
+      load_raw(row0);
+      fetch(z, 0, load_edge(z));
+      if (row0 + stride < a.rows) fetch(z + z_step, 1, load_edge(z + z_step));
+      if (row0 + 2 * stride < a.rows) edge = load_edge(z + 2 * z_step);
+      begin_entries(z, row0, 0);
+      if (row0 + stride < a.rows) load_raw(row0 + stride);
+      end_entries(z, 0);
+      announce(0);
+    }
+    for (int row = row0, buf = 0, turn = 0; row < a.rows; row += stride, z += z_step, out += out_step, buf ^= 1, turn ^= buf == 0) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&parts_in[buf], turn, wait, kErrWaitPeer))) break;
+      // ---- the whole row's sums
+      float m = -INFINITY, s1 = 0.0f, st = 0.0f;
+      for (int i = lane; i < senders; i += 32) m = fmaxf(m, inbox[buf][i].m);
+      m = warp_max(m);
+      if (m == -INFINITY) m = 0.0f;
+      for (int i = lane; i < senders; i += 32) {
+        const WarpPart p = inbox[buf][i];
+        s1 += p.s1 * Exponent{k1, m}.factor(p.m);
+        if (DUAL) st += p.st * Exponent{kt, m}.factor(p.m);
+      }
+      s1 = warp_add(s1);
+      st = DUAL ? warp_add(st) : s1;
+      const bool teach = a.weight != 0.0f && t_sum != 0.0f, has = label >= 0, active = (teach || has) && s1 != 0.0f;
+      const RowFactors f(a, g, has, teach);
+      const float c1 = (DUAL ? f.g1 : f.g1 + f.gt) * (1.0f / s1), ct = DUAL ? f.gt * (1.0f / st) : 0.0f;
+      if (lane == 0) {
+        known_row[buf] = RowKnown{m, c1, ct, active};
+        mbar_arrive(&known[buf]);
+      }
+      // ---- the place of this row's logits is free
+      if (row + 2 * stride < a.rows) {
+        fetch(z + 2 * z_step, buf, edge);
+        if (row + 3 * stride < a.rows) edge = load_edge(z + 3 * z_step);
+      }
+      const float* top_p = top_p_all + buf * a.top;
+      const float* top_z = top_z_all + buf * a.top;
+      const int* top_id = top_id_all + buf * a.top;
+      if (rank == 0) {
+        float dot = 0.0f;
+        if (teach) {
+          for (int k = lane; k < a.top; k += 32)
+            if (top_p[k] != 0.0f) dot += top_p[k] * (top_z[k] - m);
+          dot = warp_add(dot);
         }
-        if (look) {
-          __syncthreads();      // others' entries are still read
-          if (tid == 0) twice[buf] = 0;
+        if (lane == 0) store_loss(a, row, WholeRow{m, s1, st, dot, zy - m}, has, teach, t_sum, entropy);
+      }
+      // ---- the next row's label and entries are on their way while this row's gradient is written
+      const int label_now = label;
+      const float zy_now = zy, t_sum_now = t_sum;
+      const bool twice_now = twice, next = row + stride < a.rows;
+      if (next) {
+        begin_entries(z + z_step, row + stride, buf ^ 1);
+        if (row + 2 * stride < a.rows) load_raw(row + 2 * stride);
+      }
+      if (WRITE) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&written[buf], turn, wait, kErrWaitEpilogue))) break;
+        const RowPieces<T> r(z, a.V);
+        const Exponent x1{k1, m}, xt{kt, m};
+        if (active && lane == 0 && in_part(r, label_now))
+          out[label_now] = Elem<T>::from_f((c1 * exp2_approx(x1(zy_now)) - f.g1) + (DUAL ? ct * exp2_approx(xt(zy_now)) : 0.0f));
+        __syncwarp();
+        if (active && teach) {
+          for (int k = lane; k < a.top; k += 32)
+            if (in_part(r, top_id[k]))
+              store_entry<T, DUAL>(out, top_id[k], k, exp2_approx(x1(top_z[k])), DUAL ? exp2_approx(xt(top_z[k])) : 0.0f, top_id, top_p,
+                                   a.top, twice_now, c1, ct, f.g1, f.gt / t_sum_now, label_now);
         }
-        // the table of the row after next
-        for (int i = tid; i < table; i += THREADS) ids[buf * table + i] = 0;
+        __syncwarp();
+      }
+      if (next) {
+        end_entries(z + z_step, buf ^ 1);
+        announce(buf ^ 1);
       }
     }
-    if (!ok) break;
+    if (abort_word) {      // a wait ran out: the copies that are under way end before the kernel does
+      const unsigned long long t0 = globaltimer_ns();
+      for (int i = 0; i < 2; ++i)
+        while (fetched[i] && !mbar_try(&full[i], fetched[i] - 1 & 1) && globaltimer_ns() - t0 < g_wait_limit_ns) {}
+    }
   }
-  cp_async_wait<0>();
   if (parts > 1) cluster_sync_all();      // nobody leaves while parts may still be sent to it
 }
 
@@ -829,7 +861,7 @@ struct LossDevice {
 template <typename T, bool DUAL, int THREADS, int NG, bool WRITE>
 static int loss_rows_launch(const LossArgs& a, int parts, int per, cudaStream_t s) {
   auto kern = loss_rows_kernel<T, DUAL, THREADS, NG, WRITE>;
-  constexpr size_t kRaw = 2ull * THREADS * NG * 16, kSmem = kRaw + kMaxTop * 12 + 2 * loss_table_size(kMaxTop) * 4;
+  constexpr size_t kRaw = 2ull * THREADS * NG * 16, kSmem = kRaw + 2 * kMaxTop * 12 + loss_table_size(kMaxTop) * 4;
   static LossDevice known[16];
   int dev = 0;
   cudaGetDevice(&dev);
@@ -840,8 +872,8 @@ static int loss_rows_launch(const LossArgs& a, int parts, int per, cudaStream_t 
       cudaLaunchConfig_t cfg = {};
       cudaLaunchAttribute attr[1];
       cfg.gridDim = dim3(1u << i);
-      cfg.blockDim = dim3(THREADS);
-      cfg.dynamicSmemBytes = kSmem;
+      cfg.blockDim = dim3(THREADS + 32);
+      cfg.dynamicSmemBytes = kRaw;
       attr[0].id = cudaLaunchAttributeClusterDimension;
       attr[0].val.clusterDim.x = 1u << i;
       attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
@@ -855,8 +887,8 @@ static int loss_rows_launch(const LossArgs& a, int parts, int per, cudaStream_t 
   // where 71 fit, for instance, doubled the time).
   const int most = d.clusters[parts == 1 ? 0 : parts == 2 ? 1 : parts == 4 ? 2 : 3];
   const int grid = (a.rows < most ? a.rows : most) * parts;
-  const int table = WRITE && a.top > 0 ? loss_table_size(a.top) : 0;
-  launch_pdl(kern, dim3(grid), dim3(THREADS), kRaw + static_cast<size_t>(a.top) * 12 + 2ull * table * 4, s, parts, a, parts, per, table);
+  const int table = WRITE && a.top > 32 ? loss_table_size(a.top) : 0;
+  launch_pdl(kern, dim3(grid), dim3(THREADS + 32), kRaw + 24ull * a.top + 4ull * table, s, parts, a, parts, per, table);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
 
