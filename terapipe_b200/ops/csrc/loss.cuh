@@ -288,22 +288,22 @@ template <int LEFT> __device__ __forceinline__ void cp_async_wait() {
 
 // ------------------------------------------------------------------ rows held on chip
 // Logits are read once and, with WRITE, their gradient is written: what bounds the kernel is those bytes, next to it the
-// instructions of a row.  A row belongs to a cluster of 1 to 8 CTAs, each with THREADS threads that hold NG granules and one warp
-// that does everything a row needs once.  That warp has the next two rows copied into shared memory (cp.async.bulk); the others'
+// instructions of a row.  A row belongs to a cluster of 1 to 8 CTAs, each with THREADS threads that hold NG granules and two warps
+// that do what a row needs once: one has the next two rows copied into shared memory (cp.async.bulk) and adds up sums, the other
+// sees to the label and the teacher's entries.  The threads'
 // exponentials, relative to the thread's own largest logit, stay in registers in fp32 until the row's sum is known, so each is
 // computed once: two a logit and softmax would keep the exponential unit (16 a cycle and SM) busy three quarters of the time that
 // the bytes take, and two softmaxes of different temperature (DUAL) longer than that.  Without DUAL there is one
 // exponential a logit: the temperature is 1 or one of the two terms has no weight.
 //
 // There are no barriers of the CTA.  Per row, with two of each in turn: `full` (the row is in shared memory), `parts_in` (the
-// sums of all warps of the cluster have arrived, by st.async where it has several CTAs), `known` (the extra warp has added them
-// up), `written` (the CTA's part of the gradient is stored).  The label's and the teacher's elements of the gradient are then
-// stored again by the extra warp, while the others are on the next row.
-constexpr int kRowsAhead = 2;
+// sums of all warps of the cluster have arrived, by st.async where it has several CTAs, and the row's terms are known), `known`
+// (they are added up), `written` (the CTA's part of the gradient is stored).  The label's and the teacher's elements of the
+// gradient are then stored again, while the threads are on the next row.
 
 // CTAs an SM has registers for, by the exponentials a thread keeps.
 constexpr int loss_ctas_per_sm(int threads, int values) {
-  const int regs = values > 32 ? 112 : values > 16 ? 72 : 56, n = 65536 / (regs * (threads + 32));
+  const int regs = values > 32 ? 96 : values > 16 ? 64 : 48, n = 65536 / (regs * (threads + 64));
   return n < 1 ? 1 : n > 8 ? 8 : n;
 }
 
@@ -315,6 +315,12 @@ struct alignas(16) WarpPart {
 struct alignas(16) RowKnown {
   float m, c1, ct;     // largest logit; factors of exponentials relative to it
   int active;          // 0: the gradient is zero
+  float s1, st;        // sums of exponentials
+};
+// What its sums' user needs to know of a row beforehand.
+struct RowTerms {
+  float g;             // the row's factor
+  int label, teach;    // whether it has the terms
 };
 
 // Stores 16 bytes into a CTA's shared memory; they count on that CTA's barrier.  (A cluster barrier would do as
@@ -349,22 +355,27 @@ struct PartGeom {
 };
 
 template <typename T, bool DUAL, int THREADS, int NG, bool WRITE>
-__global__ void __launch_bounds__(THREADS + 32, loss_ctas_per_sm(THREADS, (WRITE ? NG : 1) * Granule<T>::N * (DUAL ? 2 : 1)))
+__global__ void __launch_bounds__(THREADS + 64, loss_ctas_per_sm(THREADS, (WRITE ? NG : 1) * Granule<T>::N * (DUAL ? 2 : 1)))
 loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
   constexpr int N = Granule<T>::N, kWarps = THREADS / 32, kSlots = THREADS * NG, kKept = WRITE ? NG : 1, kMaxParts = 8, kAhead = 4;
   extern __shared__ __align__(16) uint4 loss_smem[];
   uint4* raw = loss_smem;                                          // [2][kSlots]
-  float* top_p_all = reinterpret_cast<float*>(raw + 2 * kSlots);   // [2][top] first t, then exp((t - t_max) / T)
-  float* top_z_all = top_p_all + 2 * a.top;                        // [2][top] z, where it is needed
-  int* top_id_all = reinterpret_cast<int*>(top_z_all + 2 * a.top); // [2][top]
-  int* ids = top_id_all + 2 * a.top;                               // [table] hash table of id + 1
-  __shared__ WarpPart inbox[2][kMaxParts * kWarps + 1];
+  float* list_p_all = reinterpret_cast<float*>(raw + 2 * kSlots);    // [2][top] exp((t - t_max) / T) of the entries in this part
+  float* list_z_all = list_p_all + 2 * a.top;                        // [2][top] z
+  int* list_id_all = reinterpret_cast<int*>(list_z_all + 2 * a.top); // [2][top]
+  float* top_t = reinterpret_cast<float*>(list_id_all + 2 * a.top);  // [top] of all entries
+  int* top_id = reinterpret_cast<int*>(top_t + a.top);               // [top]
+  int* ids = top_id + a.top;                                         // [table] hash table of id + 1
+  __shared__ WarpPart inbox[2][kMaxParts * kWarps];
+  __shared__ float4 term_box[4][kMaxParts];      // rank 0's: what the parts of a row add to its loss
   __shared__ RowKnown known_row[2];
-  __shared__ uint64_t full[2], parts_in[2], known[2], written[2];
+  __shared__ RowTerms terms[2];
+  __shared__ uint64_t full[2], parts_in[2], known[2], written[2], terms_in[4];
   __shared__ int abort_word;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = parts > 1 ? cluster_ctarank() : 0;
   const int stride = gridDim.x / parts, g0 = rank * per, senders = parts * kWarps;
+  const bool teacher = a.top > 0;
   const float inv_t = 1.0f / a.temperature, kt = inv_t * kLog2e;
   // the one exponential's exponent without DUAL: z, or with a teacher alone z / T
   const float k1 = DUAL || a.weight == 0.0f ? kLog2e : kt;
@@ -377,6 +388,7 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
       mbar_init(&known[i], 1);
       mbar_init(&written[i], kWarps);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(&terms_in[i], 1);
     fence_barrier_init();
   }
   if (parts > 1) cluster_sync_all();
@@ -459,12 +471,8 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
       __syncwarp();
       if (lane == 0) mbar_arrive(&written[buf]);
     }
-  } else {
-    // ================================================================ what a row needs once
-    auto in_part = [&](const RowPieces<T>& r, int id) {
-      const int gl = static_cast<int>(static_cast<unsigned>(id + r.lead) / N) - g0;
-      return id >= 0 && gl >= 0 && gl < per;
-    };
+  } else if (warp == kWarps) {
+    // ================================================================ copies and sums
     // lanes 0 .. N - 1 have the first granule's elements, lanes 16 .. the last's, where these are not all the row's
     auto load_edge = [&](const T* z) {
       const RowPieces<T> r(z, a.V);
@@ -488,115 +496,12 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
         if (bytes) bulk_load(smem_u32(raw + buf * kSlots + from), z + ((g0 + from) * N - r.lead), bytes, &full[buf]);
       }
     };
-    // the label and the first kAhead * 32 entries of a row as they come
-    RawLabel raw_label{};
-    RawEntry raw_entry[kAhead];
-    float raw_g = 1.0f;
-    auto load_raw = [&](int row) {
-      raw_label.load(a, row);
-      if (WRITE && a.grad_loss) raw_g = a.grad_loss[row * a.ldg];
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j)
-        if (lane + 32 * j < a.top) raw_entry[j].load(a, row, lane + 32 * j);
-    };
-    // ... and of the next row as they are needed: the entries, with t_sum and whether an id occurs twice, are in half `half` of
-    // the arrays.  rank 0 has all logits, for the loss, the others those of their part.
-    int label = -1;
-    float zy = 0.0f, g = 1.0f, t_sum = 0.0f, entropy = 0.0f, z_entry[kAhead];
-    bool twice = false;
-    auto wants = [&](const RowPieces<T>& r, int id) { return id >= 0 && (rank == 0 || in_part(r, id)); };
-    auto begin_entries = [&](const T* z, int row, int half) {
-      const RowPieces<T> r(z, a.V);
-      label = raw_label.get(a);
-      g = raw_g;
-      zy = wants(r, label) ? Elem<T>::to_f(z[label]) : 0.0f;
-      for (int k0 = 0; k0 < a.top; k0 += 32 * kAhead) {
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-          const int k = k0 + lane + 32 * j;
-          if (k >= a.top) continue;
-          RawEntry e = raw_entry[j];
-          if (k0 > 0) e.load(a, row, k);
-          const int id = e.id(a);
-          top_id_all[half * a.top + k] = id;
-          top_p_all[half * a.top + k] = e.logit(a);
-          const float v = wants(r, id) ? Elem<T>::to_f(z[id]) : 0.0f;
-          if (k0 == 0) z_entry[j] = v;
-          else top_z_all[half * a.top + k] = v;
-        }
-      }
-    };
-    auto end_entries = [&](const T* z, int half) {
-      const RowPieces<T> r(z, a.V);
-      float* top_p = top_p_all + half * a.top;
-      int* top_id = top_id_all + half * a.top;
-      float t_max = -INFINITY;
-      t_sum = entropy = 0.0f;
-      twice = false;
-      if (a.top == 0) return;
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j)
-        if (lane + 32 * j < a.top) top_z_all[half * a.top + lane + 32 * j] = z_entry[j];
-      for (int k = lane; k < a.top; k += 32) t_max = fmaxf(t_max, top_p[k]);
-      t_max = warp_max(t_max);
-      if (t_max == -INFINITY) t_max = 0.0f;
-      for (int k = lane; k < a.top; k += 32) {
-        const float lt = (top_p[k] - t_max) * inv_t, p = top_id[k] >= 0 ? exp2_approx(lt * kLog2e) : 0.0f;
-        top_p[k] = p;
-        t_sum += p;
-        if (p != 0.0f) entropy += p * lt;
-      }
-      t_sum = warp_add(t_sum);
-      entropy = warp_add(entropy);
-      if (!WRITE) return;
-      if (a.top <= 32) {
-        const int id = lane < a.top ? top_id[lane] : -1;
-        const unsigned same = __match_any_sync(0xffffffffu, id);
-        twice = __any_sync(0xffffffffu, id >= 0 && (same & (same - 1)) != 0);
-      } else {
-        bool mine = false;
-        for (int i = lane; i < table; i += 32) ids[i] = 0;
-        __syncwarp();
-        for (int k = lane; k < a.top; k += 32) {
-          const int id = top_id[k];
-          if (!in_part(r, id)) continue;
-          int slot = static_cast<int>(id * 0x9e3779b1u >> 16) & (table - 1);
-          while (true) {      // (at most half of the slots are ever taken)
-            const int was = atomicCAS(&ids[slot], 0, id + 1);
-            mine |= was == id + 1;
-            if (was == 0 || was == id + 1) break;
-            slot = (slot + 1) & (table - 1);
-          }
-        }
-        twice = __any_sync(0xffffffffu, mine);
-      }
-    };
-    // rank 0 has what it needs of the row's logits: the gradient may take their place
-    auto announce = [&](int buf) {
-      __syncwarp();
-      if (parts > 1) {
-        if (lane == 0) mbar_expect_tx(&parts_in[buf], (senders + 1) * 16);
-        if (rank == 0 && lane < parts)
-          send16(mapa_u32(smem_u32(&inbox[buf][senders]), lane), mapa_u32(smem_u32(&parts_in[buf]), lane), zy, 0.0f, 0.0f);
-      } else if (lane == 0) {
-        mbar_arrive(&parts_in[buf]);
-      }
-    };
-
     T edge = Elem<T>::from_f(-INFINITY);
-    if (row0 < a.rows) {
-      load_raw(row0);
-      fetch(z, 0, load_edge(z));
-      if (row0 + stride < a.rows) fetch(z + z_step, 1, load_edge(z + z_step));
-      if (row0 + 2 * stride < a.rows) edge = load_edge(z + 2 * z_step);
-      begin_entries(z, row0, 0);
-      if (row0 + stride < a.rows) load_raw(row0 + stride);
-      end_entries(z, 0);
-      announce(0);
-    }
-    for (int row = row0, buf = 0, turn = 0; row < a.rows; row += stride, z += z_step, out += out_step, buf ^= 1, turn ^= buf == 0) {
+    if (row0 < a.rows) fetch(z, 0, load_edge(z));
+    if (row0 + stride < a.rows) fetch(z + z_step, 1, load_edge(z + z_step));
+    if (row0 + 2 * stride < a.rows) edge = load_edge(z + 2 * z_step);
+    for (int row = row0, buf = 0, turn = 0; row < a.rows; row += stride, z += z_step, buf ^= 1, turn ^= buf == 0) {
       if (!__all_sync(0xffffffffu, mbar_wait(&parts_in[buf], turn, wait, kErrWaitPeer))) break;
-      // ---- the whole row's sums
       float m = -INFINITY, s1 = 0.0f, st = 0.0f;
       for (int i = lane; i < senders; i += 32) m = fmaxf(m, inbox[buf][i].m);
       m = warp_max(m);
@@ -608,62 +513,174 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
       }
       s1 = warp_add(s1);
       st = DUAL ? warp_add(st) : s1;
-      const bool teach = a.weight != 0.0f && t_sum != 0.0f, has = label >= 0, active = (teach || has) && s1 != 0.0f;
-      const RowFactors f(a, g, has, teach);
-      const float c1 = (DUAL ? f.g1 : f.g1 + f.gt) * (1.0f / s1), ct = DUAL ? f.gt * (1.0f / st) : 0.0f;
       if (lane == 0) {
-        known_row[buf] = RowKnown{m, c1, ct, active};
+        const RowTerms t = terms[buf];
+        const RowFactors f(a, t.g, t.label, t.teach);
+        known_row[buf] = RowKnown{m, (DUAL ? f.g1 : f.g1 + f.gt) * (1.0f / s1), DUAL ? f.gt * (1.0f / st) : 0.0f,
+                                  (t.label || t.teach) && s1 != 0.0f, s1, st};
         mbar_arrive(&known[buf]);
       }
-      // ---- the place of this row's logits is free
+      // the place of this row's logits is free
       if (row + 2 * stride < a.rows) {
         fetch(z + 2 * z_step, buf, edge);
         if (row + 3 * stride < a.rows) edge = load_edge(z + 3 * z_step);
-      }
-      const float* top_p = top_p_all + buf * a.top;
-      const float* top_z = top_z_all + buf * a.top;
-      const int* top_id = top_id_all + buf * a.top;
-      if (rank == 0) {
-        float dot = 0.0f;
-        if (teach) {
-          for (int k = lane; k < a.top; k += 32)
-            if (top_p[k] != 0.0f) dot += top_p[k] * (top_z[k] - m);
-          dot = warp_add(dot);
-        }
-        if (lane == 0) store_loss(a, row, WholeRow{m, s1, st, dot, zy - m}, has, teach, t_sum, entropy);
-      }
-      // ---- the next row's label and entries are on their way while this row's gradient is written
-      const int label_now = label;
-      const float zy_now = zy, t_sum_now = t_sum;
-      const bool twice_now = twice, next = row + stride < a.rows;
-      if (next) {
-        begin_entries(z + z_step, row + stride, buf ^ 1);
-        if (row + 2 * stride < a.rows) load_raw(row + 2 * stride);
-      }
-      if (WRITE) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&written[buf], turn, wait, kErrWaitEpilogue))) break;
-        const RowPieces<T> r(z, a.V);
-        const Exponent x1{k1, m}, xt{kt, m};
-        if (active && lane == 0 && in_part(r, label_now))
-          out[label_now] = Elem<T>::from_f((c1 * exp2_approx(x1(zy_now)) - f.g1) + (DUAL ? ct * exp2_approx(xt(zy_now)) : 0.0f));
-        __syncwarp();
-        if (active && teach) {
-          for (int k = lane; k < a.top; k += 32)
-            if (in_part(r, top_id[k]))
-              store_entry<T, DUAL>(out, top_id[k], k, exp2_approx(x1(top_z[k])), DUAL ? exp2_approx(xt(top_z[k])) : 0.0f, top_id, top_p,
-                                   a.top, twice_now, c1, ct, f.g1, f.gt / t_sum_now, label_now);
-        }
-        __syncwarp();
-      }
-      if (next) {
-        end_entries(z + z_step, buf ^ 1);
-        announce(buf ^ 1);
       }
     }
     if (abort_word) {      // a wait ran out: the copies that are under way end before the kernel does
       const unsigned long long t0 = globaltimer_ns();
       for (int i = 0; i < 2; ++i)
-        while (fetched[i] && !mbar_try(&full[i], fetched[i] - 1 & 1) && globaltimer_ns() - t0 < g_wait_limit_ns) {}
+        while (fetched[i] && !mbar_try(&full[i], (fetched[i] - 1) & 1) && globaltimer_ns() - t0 < g_wait_limit_ns) {}
+    }
+  } else {
+    // ================================================================ label and teacher
+    // Entries that lie in this part are listed, in halves of the arrays for two rows in turn; their logits come from shared memory.
+    // What they and the label add to the loss goes to rank 0 when the row's sums are known.
+    auto place = [&](const RowPieces<T>& r, int id) {      // in this part: the element's number in the row's place; else -1
+      const int at = id + r.lead - g0 * N;
+      return id >= 0 && at >= 0 && at < per * N ? at : -1;
+    };
+    // the next row's label and its first kAhead * 32 entries, as they come
+    RawLabel raw_label{};
+    RawEntry raw_entry[kAhead];
+    float raw_g = 1.0f;
+    auto load_raw = [&](int row) {
+      raw_label.load(a, row);
+      if (WRITE && a.grad_loss) raw_g = a.grad_loss[row * a.ldg];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (lane + 32 * j < a.top) raw_entry[j].load(a, row, lane + 32 * j);
+    };
+    struct Row {
+      int label, listed;      // entries in the list
+      bool own, twice;        // the label is in this part; an id occurs twice in it
+      float zy, g, t_sum, entropy;
+    };
+    // Gets a row's label and entries ready and lets the row's barrier complete: with all sums in, the logits' place is free and the
+    // gradient may be stored over them.
+    auto prepare = [&](const T* z, int row, int half, int turn, Row& now) {
+      const RowPieces<T> r(z, a.V);
+      float* list_p = list_p_all + half * a.top;
+      float* list_z = list_z_all + half * a.top;
+      int* list_id = list_id_all + half * a.top;
+      now = Row{raw_label.get(a), 0, false, false, 0.0f, raw_g, 0.0f, 0.0f};
+      float t_max = -INFINITY;
+      for (int k0 = 0; k0 < a.top; k0 += 32 * kAhead) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          const int k = k0 + lane + 32 * j;
+          if (k >= a.top) continue;
+          RawEntry e = raw_entry[j];
+          if (k0 > 0) e.load(a, row, k);
+          top_id[k] = e.id(a);
+          top_t[k] = e.logit(a);
+          t_max = fmaxf(t_max, top_t[k]);
+        }
+      }
+      if (row + stride < a.rows) load_raw(row + stride);
+      if (teacher) {
+        t_max = warp_max(t_max);
+        if (t_max == -INFINITY) t_max = 0.0f;
+        for (int k0 = 0; k0 < a.top; k0 += 32) {
+          const int k = k0 + lane, id = k < a.top ? top_id[k] : -1, at = place(r, id);
+          const float lt = id >= 0 ? (top_t[k] - t_max) * inv_t : -INFINITY, p = exp2_approx(lt * kLog2e);
+          now.t_sum += p;
+          if (p != 0.0f) now.entropy += p * lt;
+          const unsigned here = __ballot_sync(0xffffffffu, at >= 0);
+          if (at >= 0) {
+            const int i = now.listed + __popc(here & ((1u << lane) - 1));
+            list_id[i] = id;
+            list_p[i] = p;
+          }
+          now.listed += __popc(here);
+        }
+        now.t_sum = warp_add(now.t_sum);
+        __syncwarp();
+      }
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[half], turn, wait, kErrWaitProducer))) return false;
+      const T* held = reinterpret_cast<const T*>(raw + half * kSlots);
+      const int label_at = place(r, now.label);
+      now.own = label_at >= 0;
+      if (now.own) now.zy = Elem<T>::to_f(held[label_at]);
+      for (int i = lane; i < now.listed; i += 32) list_z[i] = Elem<T>::to_f(held[place(r, list_id[i])]);
+      if (WRITE && now.listed <= 32) {
+        const int id = lane < now.listed ? list_id[lane] : -1;
+        const unsigned same = __match_any_sync(0xffffffffu, id);
+        now.twice = __any_sync(0xffffffffu, id >= 0 && (same & (same - 1)) != 0);
+      } else if (WRITE) {
+        bool mine = false;
+        for (int i = lane; i < table; i += 32) ids[i] = 0;
+        __syncwarp();
+        for (int i = lane; i < now.listed; i += 32) {
+          int slot = static_cast<int>(list_id[i] * 0x9e3779b1u >> 16) & (table - 1);
+          while (true) {      // (at most half of the slots are ever taken)
+            const int was = atomicCAS(&ids[slot], 0, list_id[i] + 1);
+            mine |= was == list_id[i] + 1;
+            if (was == 0 || was == list_id[i] + 1) break;
+            slot = (slot + 1) & (table - 1);
+          }
+        }
+        now.twice = __any_sync(0xffffffffu, mine);
+      }
+      if (lane == 0) terms[half] = RowTerms{now.g, now.label >= 0, a.weight != 0.0f && now.t_sum != 0.0f};
+      __syncwarp();
+      if (lane == 0) {
+        if (parts > 1) mbar_expect_tx(&parts_in[half], senders * 16);
+        else mbar_arrive(&parts_in[half]);
+      }
+      return true;
+    };
+    Row next{};
+    bool ok = true;
+    if (row0 < a.rows) {
+      load_raw(row0);
+      ok = prepare(z, row0, 0, 0, next);
+    }
+    // (the others may be up to two rows ahead of rank 0's sum of their terms: four boxes)
+    for (int row = row0, buf = 0, turn = 0, box = 0; ok && row < a.rows;
+         row += stride, z += z_step, out += out_step, buf ^= 1, turn ^= buf == 0, ++box) {
+      const Row now = next;
+      if (row + stride < a.rows && !prepare(z + z_step, row + stride, buf ^ 1, buf ? turn ^ 1 : turn, next)) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&known[buf], turn, wait, kErrWaitPeer))) break;
+      const RowKnown w = known_row[buf];
+      const bool teach = a.weight != 0.0f && now.t_sum != 0.0f, has = now.label >= 0;
+      const float* list_p = list_p_all + buf * a.top;
+      const float* list_z = list_z_all + buf * a.top;
+      const int* list_id = list_id_all + buf * a.top;
+      float dot = 0.0f, zy = now.own ? now.zy - w.m : 0.0f;
+      if (now.listed > 0) {
+        for (int i = lane; i < now.listed; i += 32)
+          if (list_p[i] != 0.0f) dot += list_p[i] * (list_z[i] - w.m);
+        dot = warp_add(dot);
+      }
+      if (parts > 1 && lane == 0) {
+        if (rank == 0) mbar_expect_tx(&terms_in[box & 3], parts * 16);
+        send16(mapa_u32(smem_u32(&term_box[box & 3][rank]), 0), mapa_u32(smem_u32(&terms_in[box & 3]), 0), dot, zy, 0.0f);
+      }
+      if (WRITE) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&written[buf], turn, wait, kErrWaitEpilogue))) break;
+        const RowFactors f(a, now.g, has, teach);
+        const Exponent x1{k1, w.m}, xt{kt, w.m};
+        if (w.active && now.own && lane == 0)
+          out[now.label] = Elem<T>::from_f((w.c1 * exp2_approx(x1(now.zy)) - f.g1) + (DUAL ? w.ct * exp2_approx(xt(now.zy)) : 0.0f));
+        if (w.active && teach && now.listed > 0) {
+          __syncwarp();
+          const float gp = f.gt / now.t_sum;
+          for (int i = lane; i < now.listed; i += 32)
+            store_entry<T, DUAL>(out, list_id[i], i, exp2_approx(x1(list_z[i])), DUAL ? exp2_approx(xt(list_z[i])) : 0.0f, list_id, list_p,
+                                 now.listed, now.twice, w.c1, w.ct, f.g1, gp, now.label);
+        }
+      }
+      if (rank == 0) {
+        if (parts > 1) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&terms_in[box & 3], box >> 2 & 1, wait, kErrWaitPeer))) break;
+          const float4 t = lane < parts ? term_box[box & 3][lane] : make_float4(0, 0, 0, 0);
+          dot = warp_add<8>(t.x);
+          zy = warp_add<8>(t.y);
+        }
+        const float entropy = teach ? warp_add(now.entropy) : 0.0f;
+        if (lane == 0) store_loss(a, row, WholeRow{w.m, w.s1, w.st, dot, zy}, has, teach, now.t_sum, entropy);
+      }
+      __syncwarp();
     }
   }
   if (parts > 1) cluster_sync_all();      // nobody leaves while parts may still be sent to it
@@ -861,7 +878,7 @@ struct LossDevice {
 template <typename T, bool DUAL, int THREADS, int NG, bool WRITE>
 static int loss_rows_launch(const LossArgs& a, int parts, int per, cudaStream_t s) {
   auto kern = loss_rows_kernel<T, DUAL, THREADS, NG, WRITE>;
-  constexpr size_t kRaw = 2ull * THREADS * NG * 16, kSmem = kRaw + 2 * kMaxTop * 12 + loss_table_size(kMaxTop) * 4;
+  constexpr size_t kRaw = 2ull * THREADS * NG * 16, kSmem = kRaw + 32 * kMaxTop + loss_table_size(kMaxTop) * 4;
   static LossDevice known[16];
   int dev = 0;
   cudaGetDevice(&dev);
@@ -872,7 +889,7 @@ static int loss_rows_launch(const LossArgs& a, int parts, int per, cudaStream_t 
       cudaLaunchConfig_t cfg = {};
       cudaLaunchAttribute attr[1];
       cfg.gridDim = dim3(1u << i);
-      cfg.blockDim = dim3(THREADS + 32);
+      cfg.blockDim = dim3(THREADS + 64);
       cfg.dynamicSmemBytes = kRaw;
       attr[0].id = cudaLaunchAttributeClusterDimension;
       attr[0].val.clusterDim.x = 1u << i;
@@ -888,7 +905,7 @@ static int loss_rows_launch(const LossArgs& a, int parts, int per, cudaStream_t 
   const int most = d.clusters[parts == 1 ? 0 : parts == 2 ? 1 : parts == 4 ? 2 : 3];
   const int grid = (a.rows < most ? a.rows : most) * parts;
   const int table = WRITE && a.top > 32 ? loss_table_size(a.top) : 0;
-  launch_pdl(kern, dim3(grid), dim3(THREADS + 32), kRaw + 24ull * a.top + 4ull * table, s, parts, a, parts, per, table);
+  launch_pdl(kern, dim3(grid), dim3(THREADS + 64), kRaw + 32ull * a.top + 4ull * table, s, parts, a, parts, per, table);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
 
