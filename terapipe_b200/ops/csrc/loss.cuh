@@ -69,11 +69,6 @@ struct RawLabel {
 struct RawEntry {
   long long v;
   uint32_t bits;
-  __device__ __forceinline__ void load(const LossArgs& a, int row, int k) {
-    v = load_id(a.tid, a.tid_at(row) + k, a.tid64);
-    const long long i = a.tlog_at(row) + k;
-    bits = a.tlog_dtype == 2 ? static_cast<const uint32_t*>(a.tlog)[i] : static_cast<const uint16_t*>(a.tlog)[i];
-  }
   __device__ __forceinline__ int id(const LossArgs& a) const { return v >= 0 && v < a.V ? static_cast<int>(v) : -1; }
   __device__ __forceinline__ float logit(const LossArgs& a) const {
     if (id(a) < 0) return -INFINITY;
@@ -82,6 +77,32 @@ struct RawEntry {
     return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
   }
 };
+// Entries k, k + 32, ... of a row, those below `top`.
+template <int COUNT> __device__ __forceinline__ void load_entries(const LossArgs& a, int row, int k, RawEntry (&e)[COUNT]) {
+  const long long at = a.tid_at(row) + k, lt = a.tlog_at(row) + k;
+  if (a.tid64) {
+    const long long* p = static_cast<const long long*>(a.tid) + at;
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j)
+      if (k + 32 * j < a.top) e[j].v = p[32 * j];
+  } else {
+    const int* p = static_cast<const int*>(a.tid) + at;
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j)
+      if (k + 32 * j < a.top) e[j].v = p[32 * j];
+  }
+  if (a.tlog_dtype == 2) {
+    const uint32_t* p = static_cast<const uint32_t*>(a.tlog) + lt;
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j)
+      if (k + 32 * j < a.top) e[j].bits = p[32 * j];
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(a.tlog) + lt;
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j)
+      if (k + 32 * j < a.top) e[j].bits = p[32 * j];
+  }
+}
 
 // A row as 16-byte pieces of memory ("granules"): granule g holds elements [g N - lead, g N - lead + N), of which those
 // outside [0, V) are not the row's.
@@ -386,7 +407,7 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
       mbar_init(&full[i], 1);
       mbar_init(&parts_in[i], parts > 1 ? 1 : kWarps + 1);      // (a launch without clusters has no st.async)
       mbar_init(&known[i], 1);
-      mbar_init(&written[i], kWarps);
+      mbar_init(&written[i], kWarps + 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&terms_in[i], 1);
     fence_barrier_init();
@@ -446,7 +467,8 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
       const bool wide = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(z)) & 15) == 0;
       if (!w.active) {
         const float o[N] = {};
-        for (int gl = tid; gl < geom.count; gl += THREADS) r.store(out, g0 + gl, o, wide && gl != geom.first && gl != geom.last);
+        for (int gl = tid; gl < geom.count; gl += THREADS)
+          if (gl != geom.first && gl != geom.last) r.store(out, g0 + gl, o, wide);
       } else {
         const float c1 = w.c1 * Exponent{k1, w.m}.factor(m_own), ct = DUAL ? w.ct * Exponent{kt, w.m}.factor(m_own) : 0.0f;
         T* o = out + ((g0 + tid) * N - r.lead);
@@ -464,8 +486,17 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
           }
           if (wide && !(k == 0 && gl == geom.first) && !(k >= kFull && gl == geom.last))
             *reinterpret_cast<uint4*>(o + k * THREADS * N) = Granule<T>::pack(v);
-          else
+        }
+        if (!wide) {
+#pragma unroll
+          for (int k = 0; k < NG; ++k) {
+            const int gl = tid + k * THREADS;
+            if ((k >= kFull && (gl >= geom.count || gl == geom.last)) || (k == 0 && gl == geom.first)) continue;
+            float v[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = DUAL ? fmaf(ct, et[k][j], c1 * e1[k][j]) : c1 * e1[k][j];
             r.store(out, g0 + gl, v, false);
+          }
         }
       }
       __syncwarp();
@@ -474,11 +505,15 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
   } else if (warp == kWarps) {
     // ================================================================ copies and sums
     // lanes 0 .. N - 1 have the first granule's elements, lanes 16 .. the last's, where these are not all the row's
-    auto load_edge = [&](const T* z) {
+    auto edge_at = [&](const T* z) {      // the lane's element, or -1
       const RowPieces<T> r(z, a.V);
       const PartGeom geom(r, g0, per);
       const int gl = lane < 16 ? geom.first : geom.last, i = (g0 + gl) * N - r.lead + (lane & 15);
-      return gl >= 0 && (lane & 15) < N && i >= 0 && i < a.V ? z[i] : Elem<T>::from_f(-INFINITY);
+      return gl >= 0 && (lane & 15) < N && i < a.V ? i : -1;
+    };
+    auto load_edge = [&](const T* z) {
+      const int i = edge_at(z);
+      return i >= 0 ? z[i] : Elem<T>::from_f(-INFINITY);
     };
     int fetched[2] = {0, 0};      // rows that each of the two places has been given
     auto fetch = [&](const T* z, int buf, T edge) {
@@ -496,11 +531,13 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
         if (bytes) bulk_load(smem_u32(raw + buf * kSlots + from), z + ((g0 + from) * N - r.lead), bytes, &full[buf]);
       }
     };
-    T edge = Elem<T>::from_f(-INFINITY);
-    if (row0 < a.rows) fetch(z, 0, load_edge(z));
-    if (row0 + stride < a.rows) fetch(z + z_step, 1, load_edge(z + z_step));
-    if (row0 + 2 * stride < a.rows) edge = load_edge(z + 2 * z_step);
-    for (int row = row0, buf = 0, turn = 0; row < a.rows; row += stride, z += z_step, buf ^= 1, turn ^= buf == 0) {
+    T edge[4];      // of this row and the next three
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      edge[i] = i < 3 && row0 + i * stride < a.rows ? load_edge(z + i * z_step) : Elem<T>::from_f(-INFINITY);
+    if (row0 < a.rows) fetch(z, 0, edge[0]);
+    if (row0 + stride < a.rows) fetch(z + z_step, 1, edge[1]);
+    for (int row = row0, buf = 0, turn = 0; row < a.rows; row += stride, z += z_step, out += out_step, buf ^= 1, turn ^= buf == 0) {
       if (!__all_sync(0xffffffffu, mbar_wait(&parts_in[buf], turn, wait, kErrWaitPeer))) break;
       float m = -INFINITY, s1 = 0.0f, st = 0.0f;
       for (int i = lane; i < senders; i += 32) m = fmaxf(m, inbox[buf][i].m);
@@ -513,18 +550,30 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
       }
       s1 = warp_add(s1);
       st = DUAL ? warp_add(st) : s1;
+      const RowTerms t = terms[buf];
+      const RowFactors f(a, t.g, t.label, t.teach);
+      const RowKnown w{m, (DUAL ? f.g1 : f.g1 + f.gt) * (1.0f / s1), DUAL ? f.gt * (1.0f / st) : 0.0f,
+                       (t.label || t.teach) && s1 != 0.0f, s1, st};
       if (lane == 0) {
-        const RowTerms t = terms[buf];
-        const RowFactors f(a, t.g, t.label, t.teach);
-        known_row[buf] = RowKnown{m, (DUAL ? f.g1 : f.g1 + f.gt) * (1.0f / s1), DUAL ? f.gt * (1.0f / st) : 0.0f,
-                                  (t.label || t.teach) && s1 != 0.0f, s1, st};
+        known_row[buf] = w;
         mbar_arrive(&known[buf]);
       }
       // the place of this row's logits is free
-      if (row + 2 * stride < a.rows) {
-        fetch(z + 2 * z_step, buf, edge);
-        if (row + 3 * stride < a.rows) edge = load_edge(z + 3 * z_step);
+      if (row + 2 * stride < a.rows) fetch(z + 2 * z_step, buf, edge[2]);
+      if (row + 3 * stride < a.rows) edge[3] = load_edge(z + 3 * z_step);
+      if (WRITE) {
+        const int i = edge_at(z);
+        if (i >= 0) {
+          const float v = Elem<T>::to_f(edge[0]);
+          float o = w.c1 * exp2_approx(Exponent{k1, m}(v));
+          if (DUAL) o += w.ct * exp2_approx(Exponent{kt, m}(v));
+          out[i] = Elem<T>::from_f(w.active ? o : 0.0f);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&written[buf]);
       }
+#pragma unroll
+      for (int i = 0; i < 3; ++i) edge[i] = edge[i + 1];
     }
     if (abort_word) {      // a wait ran out: the copies that are under way end before the kernel does
       const unsigned long long t0 = globaltimer_ns();
@@ -546,9 +595,7 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
     auto load_raw = [&](int row) {
       raw_label.load(a, row);
       if (WRITE && a.grad_loss) raw_g = a.grad_loss[row * a.ldg];
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j)
-        if (lane + 32 * j < a.top) raw_entry[j].load(a, row, lane + 32 * j);
+      if (teacher) load_entries<kAhead>(a, row, lane, raw_entry);
     };
     struct Row {
       int label, listed;      // entries in the list
@@ -565,14 +612,13 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
       now = Row{raw_label.get(a), 0, false, false, 0.0f, raw_g, 0.0f, 0.0f};
       float t_max = -INFINITY;
       for (int k0 = 0; k0 < a.top; k0 += 32 * kAhead) {
+        if (k0 > 0) load_entries<kAhead>(a, row, k0 + lane, raw_entry);
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
           const int k = k0 + lane + 32 * j;
-          if (k >= a.top) continue;
-          RawEntry e = raw_entry[j];
-          if (k0 > 0) e.load(a, row, k);
-          top_id[k] = e.id(a);
-          top_t[k] = e.logit(a);
+          if (k >= a.top) break;
+          top_id[k] = raw_entry[j].id(a);
+          top_t[k] = raw_entry[j].logit(a);
           t_max = fmaxf(t_max, top_t[k]);
         }
       }
@@ -580,6 +626,7 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
       if (teacher) {
         t_max = warp_max(t_max);
         if (t_max == -INFINITY) t_max = 0.0f;
+#pragma unroll 1
         for (int k0 = 0; k0 < a.top; k0 += 32) {
           const int k = k0 + lane, id = k < a.top ? top_id[k] : -1, at = place(r, id);
           const float lt = id >= 0 ? (top_t[k] - t_max) * inv_t : -INFINITY, p = exp2_approx(lt * kLog2e);
@@ -601,12 +648,14 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
       const int label_at = place(r, now.label);
       now.own = label_at >= 0;
       if (now.own) now.zy = Elem<T>::to_f(held[label_at]);
-      for (int i = lane; i < now.listed; i += 32) list_z[i] = Elem<T>::to_f(held[place(r, list_id[i])]);
-      if (WRITE && now.listed <= 32) {
+#pragma unroll 1
+      for (int i = lane; i < now.listed; i += 32) list_z[i] = Elem<T>::to_f(held[list_id[i] + r.lead - g0 * N]);
+      if (now.listed < 2 || !WRITE) {
+      } else if (now.listed <= 32) {
         const int id = lane < now.listed ? list_id[lane] : -1;
         const unsigned same = __match_any_sync(0xffffffffu, id);
         now.twice = __any_sync(0xffffffffu, id >= 0 && (same & (same - 1)) != 0);
-      } else if (WRITE) {
+      } else {
         bool mine = false;
         for (int i = lane; i < table; i += 32) ids[i] = 0;
         __syncwarp();
@@ -648,6 +697,7 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
       const int* list_id = list_id_all + buf * a.top;
       float dot = 0.0f, zy = now.own ? now.zy - w.m : 0.0f;
       if (now.listed > 0) {
+#pragma unroll 1
         for (int i = lane; i < now.listed; i += 32)
           if (list_p[i] != 0.0f) dot += list_p[i] * (list_z[i] - w.m);
         dot = warp_add(dot);
@@ -665,6 +715,7 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
         if (w.active && teach && now.listed > 0) {
           __syncwarp();
           const float gp = f.gt / now.t_sum;
+#pragma unroll 1
           for (int i = lane; i < now.listed; i += 32)
             store_entry<T, DUAL>(out, list_id[i], i, exp2_approx(x1(list_z[i])), DUAL ? exp2_approx(xt(list_z[i])) : 0.0f, list_id, list_p,
                                  now.listed, now.twice, w.c1, w.ct, f.g1, gp, now.label);
@@ -719,10 +770,10 @@ loss_stream_kernel(const LossArgs a, int parts, int per) {
   const float zy = own ? Elem<T>::to_f(r.row[label]) : 0.0f;
   float t_max = -INFINITY, m = -INFINITY, s1 = 0.0f, st = 0.0f;
   for (int k = tid; k < a.top; k += kThreads) {
-    RawEntry e;
-    e.load(a, row, k);
-    const int id = e.id(a);
-    const float t = e.logit(a);
+    RawEntry e[1];
+    load_entries<1>(a, row, k, e);
+    const int id = e[0].id(a);
+    const float t = e[0].logit(a);
     top_id[k] = id;
     top_p[k] = t;
     top_z[k] = in_part(id) ? Elem<T>::to_f(r.row[id]) : 0.0f;
