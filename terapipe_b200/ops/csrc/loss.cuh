@@ -193,6 +193,19 @@ __device__ __forceinline__ void granule_exp(const uint4& u, const Exponent& x, f
     e[j + 1] = exp2_approx(d.y);
   }
 }
+// x^n, n = 2, 3 or 4: with a temperature of n the exponential of z - shift is that power of the exponential of (z - shift) / n.
+__device__ __forceinline__ float2 raise2(float2 x, int n) {
+  float2 r = mul2(x, x);
+  if (n == 3) r = mul2(r, x);
+  if (n == 4) r = mul2(r, r);
+  return r;
+}
+template <int N> __device__ __forceinline__ float sum_of_powers(const float (&e)[N], int n) {
+  float2 s = raise2(make_float2(e[0], e[1]), n);
+#pragma unroll
+  for (int j = 2; j < N; j += 2) s = add2(s, raise2(make_float2(e[j], e[j + 1]), n));
+  return s.x + s.y;
+}
 template <int N> __device__ __forceinline__ float sum_of(const float (&e)[N]) {
   float2 s = make_float2(e[0], e[1]);
 #pragma unroll
@@ -336,12 +349,12 @@ struct alignas(16) WarpPart {
 struct alignas(16) RowKnown {
   float m, c1, ct;     // largest logit; factors of exponentials relative to it
   int active;          // 0: the gradient is zero
-  float s1, st;        // sums of exponentials
 };
-// What its sums' user needs to know of a row beforehand.
+// What is known of a row before its sums: its label and entries.
 struct RowTerms {
-  float g;             // the row's factor
-  int label, teach;    // whether it has the terms
+  float g, zy, t_sum, entropy;      // the row's factor; z_y if the label is in this part; sums over all entries
+  int label, listed;                // -1: no label; entries listed
+  bool teach, own, twice;           // the row has the teacher's term; the label is in this part; an id occurs twice in it
 };
 
 // Stores 16 bytes into a CTA's shared memory; they count on that CTA's barrier.  (A cluster barrier would do as
@@ -375,28 +388,30 @@ struct PartGeom {
   }
 };
 
-template <typename T, bool DUAL, int THREADS, int NG, bool WRITE>
-__global__ void __launch_bounds__(THREADS + 64, loss_ctas_per_sm(THREADS, (WRITE ? NG : 1) * Granule<T>::N * (DUAL ? 2 : 1)))
+template <typename T, int SOFT, int THREADS, int NG, bool WRITE>
+__global__ void __launch_bounds__(THREADS + 64, loss_ctas_per_sm(THREADS, (WRITE ? NG : 1) * Granule<T>::N * (SOFT == 1 ? 2 : 1)))
 loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
+  constexpr bool DUAL = SOFT != 0, POWER = SOFT == 2;
   constexpr int N = Granule<T>::N, kWarps = THREADS / 32, kSlots = THREADS * NG, kKept = WRITE ? NG : 1, kMaxParts = 8, kAhead = 4;
   extern __shared__ __align__(16) uint4 loss_smem[];
   uint4* raw = loss_smem;                                          // [2][kSlots]
-  float* list_p_all = reinterpret_cast<float*>(raw + 2 * kSlots);    // [2][top] exp((t - t_max) / T) of the entries in this part
-  float* list_z_all = list_p_all + 2 * a.top;                        // [2][top] z
-  int* list_id_all = reinterpret_cast<int*>(list_z_all + 2 * a.top); // [2][top]
-  float* top_t = reinterpret_cast<float*>(list_id_all + 2 * a.top);  // [top] of all entries
+  float* list_p_all = reinterpret_cast<float*>(raw + 2 * kSlots);    // [4][top] exp((t - t_max) / T) of the entries in this part
+  float* list_z_all = list_p_all + 4 * a.top;                        // [4][top] z
+  int* list_id_all = reinterpret_cast<int*>(list_z_all + 4 * a.top); // [4][top]
+  float* top_t = reinterpret_cast<float*>(list_id_all + 4 * a.top);  // [top] of all entries
   int* top_id = reinterpret_cast<int*>(top_t + a.top);               // [top]
   int* ids = top_id + a.top;                                         // [table] hash table of id + 1
   __shared__ WarpPart inbox[2][kMaxParts * kWarps];
   __shared__ float4 term_box[4][kMaxParts];      // rank 0's: what the parts of a row add to its loss
   __shared__ RowKnown known_row[2];
-  __shared__ RowTerms terms[2];
+  __shared__ RowTerms terms[4];
   __shared__ uint64_t full[2], parts_in[2], known[2], written[2], terms_in[4];
   __shared__ int abort_word;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = parts > 1 ? cluster_ctarank() : 0;
   const int stride = gridDim.x / parts, g0 = rank * per, senders = parts * kWarps;
   const bool teacher = a.top > 0;
+  const int power = static_cast<int>(a.temperature);
   const float inv_t = 1.0f / a.temperature, kt = inv_t * kLog2e;
   // the one exponential's exponent without DUAL: z, or with a teacher alone z / T
   const float k1 = DUAL || a.weight == 0.0f ? kLog2e : kt;
@@ -407,7 +422,7 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
       mbar_init(&full[i], 1);
       mbar_init(&parts_in[i], parts > 1 ? 1 : kWarps + 1);      // (a launch without clusters has no st.async)
       mbar_init(&known[i], 1);
-      mbar_init(&written[i], kWarps + 1);
+      mbar_init(&written[i], kWarps);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&terms_in[i], 1);
     fence_barrier_init();
@@ -435,17 +450,21 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
         if (k < kFull || tid + k * THREADS < geom.count) largest.add(mine[k * THREADS]);
       const float m_own = largest.get(), shift = m_own == -INFINITY ? 0.0f : m_own;
       const Exponent x1{k1, shift}, xt{kt, shift};
-      float e1[kKept][N], et[DUAL ? kKept : 1][N], s1 = 0.0f, st = 0.0f;
+      float e1[POWER ? 1 : kKept][N], et[DUAL ? kKept : 1][N], s1 = 0.0f, st = 0.0f;
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
         const int kept = WRITE ? k : 0;
         if (k >= kFull && tid + k * THREADS >= geom.count) continue;
         const uint4 u = mine[k * THREADS];
-        granule_exp<T>(u, x1, e1[kept]);
-        s1 += sum_of<N>(e1[kept]);
         if (DUAL) {
           granule_exp<T>(u, xt, et[kept]);
           st += sum_of<N>(et[kept]);
+        }
+        if (POWER) {
+          s1 += sum_of_powers<N>(et[kept], power);
+        } else {
+          granule_exp<T>(u, x1, e1[kept]);
+          s1 += sum_of<N>(e1[kept]);
         }
       }
       const float m_warp = warp_max(m_own), m_from = m_warp == -INFINITY ? 0.0f : m_warp;
@@ -479,8 +498,9 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
           float v[N];
 #pragma unroll
           for (int j = 0; j < N; j += 2) {
-            float2 d = mul2(make_float2(e1[k][j], e1[k][j + 1]), dup2(c1));
-            if (DUAL) d = fma2(make_float2(et[k][j], et[k][j + 1]), dup2(ct), d);
+            const float2 d2 = DUAL ? make_float2(et[k][j], et[k][j + 1]) : make_float2(0.0f, 0.0f);
+            float2 d = mul2(POWER ? raise2(d2, power) : make_float2(e1[POWER ? 0 : k][j], e1[POWER ? 0 : k][j + 1]), dup2(c1));
+            if (DUAL) d = fma2(d2, dup2(ct), d);
             v[j] = d.x;
             v[j + 1] = d.y;
           }
@@ -494,7 +514,10 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
             if ((k >= kFull && (gl >= geom.count || gl == geom.last)) || (k == 0 && gl == geom.first)) continue;
             float v[N];
 #pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = DUAL ? fmaf(ct, et[k][j], c1 * e1[k][j]) : c1 * e1[k][j];
+            for (int j = 0; j < N; ++j) {
+              const float vt = DUAL ? et[k][j] : 0.0f, v1 = POWER ? raise2(make_float2(vt, vt), power).x : e1[POWER ? 0 : k][j];
+              v[j] = DUAL ? fmaf(ct, vt, c1 * v1) : c1 * v1;
+            }
             r.store(out, g0 + gl, v, false);
           }
         }
@@ -537,8 +560,24 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
       edge[i] = i < 3 && row0 + i * stride < a.rows ? load_edge(z + i * z_step) : Elem<T>::from_f(-INFINITY);
     if (row0 < a.rows) fetch(z, 0, edge[0]);
     if (row0 + stride < a.rows) fetch(z + z_step, 1, edge[1]);
-    for (int row = row0, buf = 0, turn = 0; row < a.rows; row += stride, z += z_step, out += out_step, buf ^= 1, turn ^= buf == 0) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&parts_in[buf], turn, wait, kErrWaitPeer))) break;
+    // A row's loss is stored when the next row's sums are known: what the other parts add to it has arrived long before.
+    // (They may be two rows ahead: four boxes.)
+    WholeRow whole{};
+    RowTerms t_last{};
+    auto finish_loss = [&](int row, int n) {
+      if (parts > 1) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&terms_in[n & 3], n >> 2 & 1, wait, kErrWaitPeer))) return false;
+        const float4 v = lane < parts ? term_box[n & 3][lane] : make_float4(0, 0, 0, 0);
+        whole.dot = warp_add<8>(v.x);
+        whole.zy = warp_add<8>(v.y);
+      }
+      if (lane == 0) store_loss(a, row, whole, t_last.label >= 0, t_last.teach, t_last.t_sum, t_last.entropy);
+      return true;
+    };
+    int n = 0;      // rows done
+    bool ok = true;
+    for (int row = row0, buf = 0, turn = 0; row < a.rows; row += stride, z += z_step, out += out_step, buf ^= 1, turn ^= buf == 0, ++n) {
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(&parts_in[buf], turn, wait, kErrWaitPeer)))) break;
       float m = -INFINITY, s1 = 0.0f, st = 0.0f;
       for (int i = lane; i < senders; i += 32) m = fmaxf(m, inbox[buf][i].m);
       m = warp_max(m);
@@ -550,31 +589,60 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
       }
       s1 = warp_add(s1);
       st = DUAL ? warp_add(st) : s1;
-      const RowTerms t = terms[buf];
-      const RowFactors f(a, t.g, t.label, t.teach);
-      const RowKnown w{m, (DUAL ? f.g1 : f.g1 + f.gt) * (1.0f / s1), DUAL ? f.gt * (1.0f / st) : 0.0f,
-                       (t.label || t.teach) && s1 != 0.0f, s1, st};
+      const RowTerms t = terms[n & 3];
+      const RowFactors f(a, t.g, t.label >= 0, t.teach);
+      const float c1 = (DUAL ? f.g1 : f.g1 + f.gt) * (1.0f / s1), ct = DUAL ? f.gt * (1.0f / st) : 0.0f;
+      const bool active = (t.label >= 0 || t.teach) && s1 != 0.0f;
       if (lane == 0) {
-        known_row[buf] = w;
+        known_row[buf] = RowKnown{m, c1, ct, active};
         mbar_arrive(&known[buf]);
       }
       // the place of this row's logits is free
       if (row + 2 * stride < a.rows) fetch(z + 2 * z_step, buf, edge[2]);
       if (row + 3 * stride < a.rows) edge[3] = load_edge(z + 3 * z_step);
+      if (rank == 0 && n > 0 && !(ok = finish_loss(row - stride, n - 1))) break;
+      const float* list_p = list_p_all + (n & 3) * a.top;
+      const float* list_z = list_z_all + (n & 3) * a.top;
+      const int* list_id = list_id_all + (n & 3) * a.top;
+      float dot = 0.0f;
+      const float zy = t.own ? t.zy - m : 0.0f;
+      if (t.listed > 0) {
+#pragma unroll 1
+        for (int i = lane; i < t.listed; i += 32)
+          if (list_p[i] != 0.0f) dot += list_p[i] * (list_z[i] - m);
+        dot = warp_add(dot);
+      }
+      if (parts > 1 && lane == 0) {
+        if (rank == 0) mbar_expect_tx(&terms_in[n & 3], parts * 16);
+        send16(mapa_u32(smem_u32(&term_box[n & 3][rank]), 0), mapa_u32(smem_u32(&terms_in[n & 3]), 0), dot, zy, 0.0f);
+      }
+      whole = WholeRow{m, s1, st, dot, zy};
+      t_last = t;
       if (WRITE) {
+        const Exponent x1{k1, m}, xt{kt, m};
         const int i = edge_at(z);
         if (i >= 0) {
           const float v = Elem<T>::to_f(edge[0]);
-          float o = w.c1 * exp2_approx(Exponent{k1, m}(v));
-          if (DUAL) o += w.ct * exp2_approx(Exponent{kt, m}(v));
-          out[i] = Elem<T>::from_f(w.active ? o : 0.0f);
+          out[i] = Elem<T>::from_f(active ? c1 * exp2_approx(x1(v)) + (DUAL ? ct * exp2_approx(xt(v)) : 0.0f) : 0.0f);
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&written[buf]);
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&written[buf], turn, wait, kErrWaitEpilogue)))) break;
+        if (active && t.own && lane == 0)
+          out[t.label] = Elem<T>::from_f((c1 * exp2_approx(x1(t.zy)) - f.g1) + (DUAL ? ct * exp2_approx(xt(t.zy)) : 0.0f));
+        if (active && t.teach && t.listed > 0) {
+          __syncwarp();
+          const float gp = f.gt / t.t_sum;
+#pragma unroll 1
+          for (int i = lane; i < t.listed; i += 32)
+            store_entry<T, DUAL>(out, list_id[i], i, exp2_approx(x1(list_z[i])), DUAL ? exp2_approx(xt(list_z[i])) : 0.0f, list_id, list_p,
+                                 t.listed, t.twice, c1, ct, f.g1, gp, t.label);
+        }
+        __syncwarp();
       }
 #pragma unroll
       for (int i = 0; i < 3; ++i) edge[i] = edge[i + 1];
     }
+    if (ok && rank == 0 && n > 0) finish_loss(row0 + (n - 1) * stride, n - 1);
     if (abort_word) {      // a wait ran out: the copies that are under way end before the kernel does
       const unsigned long long t0 = globaltimer_ns();
       for (int i = 0; i < 2; ++i)
@@ -582,8 +650,7 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
     }
   } else {
     // ================================================================ label and teacher
-    // Entries that lie in this part are listed, in halves of the arrays for two rows in turn; their logits come from shared memory.
-    // What they and the label add to the loss goes to rank 0 when the row's sums are known.
+    // Entries that lie in this part are listed, in quarters of the arrays for four rows in turn; their logits come from shared memory.
     auto place = [&](const RowPieces<T>& r, int id) {      // in this part: the element's number in the row's place; else -1
       const int at = id + r.lead - g0 * N;
       return id >= 0 && at >= 0 && at < per * N ? at : -1;
@@ -597,19 +664,18 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
       if (WRITE && a.grad_loss) raw_g = a.grad_loss[row * a.ldg];
       if (teacher) load_entries<kAhead>(a, row, lane, raw_entry);
     };
-    struct Row {
-      int label, listed;      // entries in the list
-      bool own, twice;        // the label is in this part; an id occurs twice in it
-      float zy, g, t_sum, entropy;
-    };
     // Gets a row's label and entries ready and lets the row's barrier complete: with all sums in, the logits' place is free and the
     // gradient may be stored over them.
-    auto prepare = [&](const T* z, int row, int half, int turn, Row& now) {
+    // (A row's list is read until its gradient is stored, which is before the sums of the next row are known.)
+    load_raw(row0 < a.rows ? row0 : 0);
+    int n = 0;
+    for (int row = row0, half = 0, turn = 0; row < a.rows; row += stride, z += z_step, half ^= 1, turn ^= half == 0, ++n) {
+      if (n >= 2 && !__all_sync(0xffffffffu, mbar_wait(&known[half], turn ^ 1, wait, kErrWaitPeer))) break;      // of two rows before
       const RowPieces<T> r(z, a.V);
-      float* list_p = list_p_all + half * a.top;
-      float* list_z = list_z_all + half * a.top;
-      int* list_id = list_id_all + half * a.top;
-      now = Row{raw_label.get(a), 0, false, false, 0.0f, raw_g, 0.0f, 0.0f};
+      float* list_p = list_p_all + (n & 3) * a.top;
+      float* list_z = list_z_all + (n & 3) * a.top;
+      int* list_id = list_id_all + (n & 3) * a.top;
+      RowTerms now{raw_g, 0.0f, 0.0f, 0.0f, raw_label.get(a), 0, false, false, false};
       float t_max = -INFINITY;
       for (int k0 = 0; k0 < a.top; k0 += 32 * kAhead) {
         if (k0 > 0) load_entries<kAhead>(a, row, k0 + lane, raw_entry);
@@ -643,7 +709,7 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
         now.t_sum = warp_add(now.t_sum);
         __syncwarp();
       }
-      if (!__all_sync(0xffffffffu, mbar_wait(&full[half], turn, wait, kErrWaitProducer))) return false;
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[half], turn, wait, kErrWaitProducer))) break;
       const T* held = reinterpret_cast<const T*>(raw + half * kSlots);
       const int label_at = place(r, now.label);
       now.own = label_at >= 0;
@@ -670,68 +736,14 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
         }
         now.twice = __any_sync(0xffffffffu, mine);
       }
-      if (lane == 0) terms[half] = RowTerms{now.g, now.label >= 0, a.weight != 0.0f && now.t_sum != 0.0f};
+      now.teach = a.weight != 0.0f && now.t_sum != 0.0f;
+      if (rank == 0) now.entropy = warp_add(now.entropy);
       __syncwarp();
       if (lane == 0) {
+        terms[n & 3] = now;
         if (parts > 1) mbar_expect_tx(&parts_in[half], senders * 16);
         else mbar_arrive(&parts_in[half]);
       }
-      return true;
-    };
-    Row next{};
-    bool ok = true;
-    if (row0 < a.rows) {
-      load_raw(row0);
-      ok = prepare(z, row0, 0, 0, next);
-    }
-    // (the others may be up to two rows ahead of rank 0's sum of their terms: four boxes)
-    for (int row = row0, buf = 0, turn = 0, box = 0; ok && row < a.rows;
-         row += stride, z += z_step, out += out_step, buf ^= 1, turn ^= buf == 0, ++box) {
-      const Row now = next;
-      if (row + stride < a.rows && !prepare(z + z_step, row + stride, buf ^ 1, buf ? turn ^ 1 : turn, next)) break;
-      if (!__all_sync(0xffffffffu, mbar_wait(&known[buf], turn, wait, kErrWaitPeer))) break;
-      const RowKnown w = known_row[buf];
-      const bool teach = a.weight != 0.0f && now.t_sum != 0.0f, has = now.label >= 0;
-      const float* list_p = list_p_all + buf * a.top;
-      const float* list_z = list_z_all + buf * a.top;
-      const int* list_id = list_id_all + buf * a.top;
-      float dot = 0.0f, zy = now.own ? now.zy - w.m : 0.0f;
-      if (now.listed > 0) {
-#pragma unroll 1
-        for (int i = lane; i < now.listed; i += 32)
-          if (list_p[i] != 0.0f) dot += list_p[i] * (list_z[i] - w.m);
-        dot = warp_add(dot);
-      }
-      if (parts > 1 && lane == 0) {
-        if (rank == 0) mbar_expect_tx(&terms_in[box & 3], parts * 16);
-        send16(mapa_u32(smem_u32(&term_box[box & 3][rank]), 0), mapa_u32(smem_u32(&terms_in[box & 3]), 0), dot, zy, 0.0f);
-      }
-      if (WRITE) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&written[buf], turn, wait, kErrWaitEpilogue))) break;
-        const RowFactors f(a, now.g, has, teach);
-        const Exponent x1{k1, w.m}, xt{kt, w.m};
-        if (w.active && now.own && lane == 0)
-          out[now.label] = Elem<T>::from_f((w.c1 * exp2_approx(x1(now.zy)) - f.g1) + (DUAL ? w.ct * exp2_approx(xt(now.zy)) : 0.0f));
-        if (w.active && teach && now.listed > 0) {
-          __syncwarp();
-          const float gp = f.gt / now.t_sum;
-#pragma unroll 1
-          for (int i = lane; i < now.listed; i += 32)
-            store_entry<T, DUAL>(out, list_id[i], i, exp2_approx(x1(list_z[i])), DUAL ? exp2_approx(xt(list_z[i])) : 0.0f, list_id, list_p,
-                                 now.listed, now.twice, w.c1, w.ct, f.g1, gp, now.label);
-        }
-      }
-      if (rank == 0) {
-        if (parts > 1) {
-          if (!__all_sync(0xffffffffu, mbar_wait(&terms_in[box & 3], box >> 2 & 1, wait, kErrWaitPeer))) break;
-          const float4 t = lane < parts ? term_box[box & 3][lane] : make_float4(0, 0, 0, 0);
-          dot = warp_add<8>(t.x);
-          zy = warp_add<8>(t.y);
-        }
-        const float entropy = teach ? warp_add(now.entropy) : 0.0f;
-        if (lane == 0) store_loss(a, row, WholeRow{w.m, w.s1, w.st, dot, zy}, has, teach, now.t_sum, entropy);
-      }
-      __syncwarp();
     }
   }
   if (parts > 1) cluster_sync_all();      // nobody leaves while parts may still be sent to it
@@ -740,9 +752,10 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
 // ------------------------------------------------------------------ rows read twice
 // The gradient from a forward pass's statistics (MODE 2), and rows that a cluster cannot hold (1 and 3: the second read is
 // served by L2 where it can).  A CTA per part of a row; the parts of a row form a cluster where their sums have to be joined.
-template <typename T, bool DUAL, int MODE>
+template <typename T, int SOFT, int MODE>
 __global__ void __launch_bounds__(512, 2)
 loss_stream_kernel(const LossArgs a, int parts, int per) {
+  constexpr bool DUAL = SOFT != 0, POWER = SOFT == 2;
   constexpr int N = Granule<T>::N, kWarps = 16, kThreads = 512, kAhead = 4;
   extern __shared__ __align__(16) uint4 loss_smem[];
   float* top_p = reinterpret_cast<float*>(loss_smem);
@@ -755,6 +768,7 @@ loss_stream_kernel(const LossArgs a, int parts, int per) {
   const float inv_t = 1.0f / a.temperature, kt = inv_t * kLog2e;
   const float k1 = DUAL || a.weight == 0.0f ? kLog2e : kt;
   const bool teacher = a.top > 0;
+  const int power = static_cast<int>(a.temperature);
   pdl_wait();
   const RowPieces<T> r(static_cast<const T*>(a.logits) + row * a.ld, a.V);
   const int g0 = static_cast<int>(min(static_cast<long long>(rank) * per, static_cast<long long>(r.count)));
@@ -800,12 +814,16 @@ loss_stream_kernel(const LossArgs a, int parts, int per) {
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         if (g + k * kThreads >= g1) continue;
-        float e[N];
-        granule_exp<T>(u[k], x1, e);
-        s1 += sum_of<N>(e);
+        float e[N], e2[N];
         if (DUAL) {
-          granule_exp<T>(u[k], xt, e);
-          st += sum_of<N>(e);
+          granule_exp<T>(u[k], xt, e2);
+          st += sum_of<N>(e2);
+        }
+        if (POWER) {
+          s1 += sum_of_powers<N>(e2, power);
+        } else {
+          granule_exp<T>(u[k], x1, e);
+          s1 += sum_of<N>(e);
         }
       }
     }
@@ -893,15 +911,15 @@ loss_stream_kernel(const LossArgs a, int parts, int per) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       if (g + k * kThreads >= g1) continue;
-      float e[N] = {}, o[N] = {};
+      float o[N] = {};
       if (!zero) {
-        granule_exp<T>(u[k], x1, e);
+        float e[N], e2[N];
+        if (DUAL) granule_exp<T>(u[k], xt, e2);
+        if (!POWER) granule_exp<T>(u[k], x1, e);
 #pragma unroll
-        for (int j = 0; j < N; ++j) o[j] = c1 * e[j];
-        if (DUAL) {
-          granule_exp<T>(u[k], xt, e);
-#pragma unroll
-          for (int j = 0; j < N; ++j) o[j] += ct * e[j];
+        for (int j = 0; j < N; ++j) {
+          const float v1 = POWER ? raise2(make_float2(e2[j], e2[j]), power).x : e[j];
+          o[j] = DUAL ? fmaf(ct, e2[j], c1 * v1) : c1 * v1;
         }
       }
       r.store(out, g + k * kThreads, o, wide && !r.edge(g + k * kThreads));
@@ -926,10 +944,10 @@ struct LossDevice {
   bool ready;
 };
 
-template <typename T, bool DUAL, int THREADS, int NG, bool WRITE>
+template <typename T, int SOFT, int THREADS, int NG, bool WRITE>
 static int loss_rows_launch(const LossArgs& a, int parts, int per, cudaStream_t s) {
-  auto kern = loss_rows_kernel<T, DUAL, THREADS, NG, WRITE>;
-  constexpr size_t kRaw = 2ull * THREADS * NG * 16, kSmem = kRaw + 32 * kMaxTop + loss_table_size(kMaxTop) * 4;
+  auto kern = loss_rows_kernel<T, SOFT, THREADS, NG, WRITE>;
+  constexpr size_t kRaw = 2ull * THREADS * NG * 16, kSmem = kRaw + 56 * kMaxTop + loss_table_size(kMaxTop) * 4;
   static LossDevice known[16];
   int dev = 0;
   cudaGetDevice(&dev);
@@ -956,54 +974,57 @@ static int loss_rows_launch(const LossArgs& a, int parts, int per, cudaStream_t 
   const int most = d.clusters[parts == 1 ? 0 : parts == 2 ? 1 : parts == 4 ? 2 : 3];
   const int grid = (a.rows < most ? a.rows : most) * parts;
   const int table = WRITE && a.top > 32 ? loss_table_size(a.top) : 0;
-  launch_pdl(kern, dim3(grid), dim3(THREADS + 64), kRaw + 32ull * a.top + 4ull * table, s, parts, a, parts, per, table);
+  launch_pdl(kern, dim3(grid), dim3(THREADS + 64), kRaw + 56ull * a.top + 4ull * table, s, parts, a, parts, per, table);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
 
-template <typename T, bool DUAL, int MODE> static int loss_stream_launch(const LossArgs& a, int parts, int per, cudaStream_t s) {
+template <typename T, int SOFT, int MODE> static int loss_stream_launch(const LossArgs& a, int parts, int per, cudaStream_t s) {
   const long long grid = static_cast<long long>(a.rows) * parts;
   if (grid > 0x7fffffffll) return kErrTooLarge;
-  launch_pdl(loss_stream_kernel<T, DUAL, MODE>, dim3(static_cast<unsigned>(grid)), dim3(512), static_cast<size_t>(a.top) * 12, s,
+  launch_pdl(loss_stream_kernel<T, SOFT, MODE>, dim3(static_cast<unsigned>(grid)), dim3(512), static_cast<size_t>(a.top) * 12, s,
              MODE & kLossFwd ? parts : 1, a, parts, per);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
 
 // The kernel for `per` granules a part at THREADS threads: the parts of a row differ by at most 8 granules (its last part, and the
 // granule more that an offset from a 16-byte boundary needs), so that all but the last two granules a thread are full.
-template <typename T, bool DUAL, int THREADS, int NG, bool WRITE>
+template <typename T, int SOFT, int THREADS, int NG, bool WRITE>
 static int loss_rows_fit(const LossArgs& a, int parts, int per, cudaStream_t s) {
   if constexpr (NG > 1) {
-    if (per <= THREADS * (NG - 1)) return loss_rows_fit<T, DUAL, THREADS, NG - 1, WRITE>(a, parts, per, s);
+    if (per <= THREADS * (NG - 1)) return loss_rows_fit<T, SOFT, THREADS, NG - 1, WRITE>(a, parts, per, s);
   }
-  return loss_rows_launch<T, DUAL, THREADS, NG, WRITE>(a, parts, per, s);
+  return loss_rows_launch<T, SOFT, THREADS, NG, WRITE>(a, parts, per, s);
 }
 
-template <typename T, bool DUAL, bool WRITE> static int loss_choose(const LossArgs& a, cudaStream_t s) {
-  constexpr int N = Granule<T>::N, kMost = DUAL ? 4 : 8;      // granules a thread: registers for their exponentials
+template <typename T, int SOFT, bool WRITE> static int loss_choose(const LossArgs& a, cudaStream_t s) {
+  constexpr int N = Granule<T>::N, kMost = SOFT == 1 ? 4 : 8;      // granules a thread: registers for their exponentials
   // granules of the longest row: rows on different offsets from a 16-byte boundary may need one more
   const bool same = a.rows == 1 || a.ld * static_cast<long long>(sizeof(T)) % 16 == 0;
   const long long lead = same ? (reinterpret_cast<uintptr_t>(a.logits) & 15) / sizeof(T) : N - 1;
   const long long granules = (a.V + lead + N - 1) / N;
-  if (granules <= 128 * 4) return loss_rows_fit<T, DUAL, 128, 4, WRITE>(a, 1, static_cast<int>(granules), s);
+  if (granules <= 128 * 4) return loss_rows_fit<T, SOFT, 128, 4, WRITE>(a, 1, static_cast<int>(granules), s);
   int parts = 1;
   while (parts < 8 && granules > parts * 256ll * kMost) parts *= 2;
   while (parts < 8 && a.rows * parts * 2ll <= num_sms() && granules > parts * 512ll) parts *= 2;
   const int per = static_cast<int>((granules + parts - 1) / parts);
-  if (per <= 256 * kMost) return loss_rows_fit<T, DUAL, 256, kMost, WRITE>(a, parts, per, s);
-  if (per <= 512 * kMost) return loss_rows_fit<T, DUAL, 512, kMost, WRITE>(a, parts, per, s);
-  return loss_stream_launch<T, DUAL, kLossFwd | (WRITE ? kLossBwd : 0)>(a, parts, per, s);
+  if (per <= 256 * kMost) return loss_rows_fit<T, SOFT, 256, kMost, WRITE>(a, parts, per, s);
+  if (per <= 512 * kMost) return loss_rows_fit<T, SOFT, 512, kMost, WRITE>(a, parts, per, s);
+  return loss_stream_launch<T, SOFT, kLossFwd | (WRITE ? kLossBwd : 0)>(a, parts, per, s);
 }
 
-template <typename T, bool DUAL> static int loss_mode(const LossArgs& a, int mode, cudaStream_t s) {
-  if (mode == kLossFwd) return loss_choose<T, DUAL, false>(a, s);
-  if (mode == (kLossFwd | kLossBwd)) return loss_choose<T, DUAL, true>(a, s);
+template <typename T, int SOFT> static int loss_mode(const LossArgs& a, int mode, cudaStream_t s) {
+  if (mode == kLossFwd) return loss_choose<T, SOFT, false>(a, s);
+  if (mode == (kLossFwd | kLossBwd)) return loss_choose<T, SOFT, true>(a, s);
   const int per = 2048;
   const long long granules = (a.V + 2ll * Granule<T>::N - 2) / Granule<T>::N;
-  return loss_stream_launch<T, DUAL, kLossBwd>(a, static_cast<int>(granules > per ? (granules + per - 1) / per : 1), per, s);
+  return loss_stream_launch<T, SOFT, kLossBwd>(a, static_cast<int>(granules > per ? (granules + per - 1) / per : 1), per, s);
 }
 
 template <typename T> static int loss_launch(const LossArgs& a, int mode, cudaStream_t s) {
-  if (a.weight > 0.0f && a.weight < 1.0f && a.top > 0 && a.labels && a.temperature != 1.0f) return loss_mode<T, true>(a, mode, s);
-  return loss_mode<T, false>(a, mode, s);
+  if (a.weight > 0.0f && a.weight < 1.0f && a.top > 0 && a.labels && a.temperature != 1.0f) {
+    if (a.temperature == 2.0f || a.temperature == 3.0f || a.temperature == 4.0f) return loss_mode<T, 2>(a, mode, s);
+    return loss_mode<T, 1>(a, mode, s);
+  }
+  return loss_mode<T, 0>(a, mode, s);
 }
 }  // namespace tp
