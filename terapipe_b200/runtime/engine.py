@@ -259,6 +259,10 @@ class StageEngine:
         self._alloc_activations()
         self.status = F.status_word(dev)
         self.loss_buf = torch.zeros(1, dtype=torch.float32, device=dev)
+        # What a language model has in front of its layers and behind them (runtime/token_trainer.py): an object whose
+        # begin() writes X[0], whose head() reads the output and writes dY, and whose finish(update) reads dA.  Without
+        # one the input is set_input's and the loss the mean of the output.
+        self.ends = None
         self._graph = self._add_graph = None    # of the usual step, of one that adds to gradients left in the buffer
         self._add_eager = False
         self._cap_stream = None
@@ -1090,7 +1094,9 @@ class StageEngine:
                     lo, hi = self._link_rows(sl)
                     sends.append(dist.isend(self.X[self.n_layers][lo:hi],
                                             mpu.get_pipeline_next_rank(), group=self._link_next))
-        if self.is_last:
+        if self.ends is not None:
+            self.ends.head()
+        elif self.is_last:
             self.loss_buf.copy_(self.X[self.n_layers].sum(dtype=torch.float32))
         recvs = self._post_recvs(False) if (pipelined and not self.is_last) else None
         if merged:
@@ -1215,6 +1221,8 @@ class StageEngine:
             self._group_barrier(1)
         self._dp_overlap = bool(update and self.dp > 1 and self.dp_overlap)
         self._dp_works = None
+        if self.ends is not None:
+            self.ends.begin()
         fused_update = update and (self._updates_in_products if fused is None else fused)
         self._forward_backward("update" if fused_update else "add" if update or self.dp > 1 or self.sp else "assign")
         if update and not (self.dp_sym is not None and self._dp_overlap and not self.sp):
@@ -1225,6 +1233,8 @@ class StageEngine:
                 self._reduce_and_update(fused_update)
             if not torch.cuda.is_current_stream_capturing():
                 self._grads.cleared()
+        if self.ends is not None:
+            self.ends.finish(update)
 
     def set_input(self, x: torch.Tensor) -> None:
         """Copy this replica's ``[L, B, H]`` input into the stage-0 activation buffer.  Rows are

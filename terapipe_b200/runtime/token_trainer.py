@@ -1,0 +1,150 @@
+"""A language model on one GPU: tokens in, cross entropy or distillation out.
+
+    trainer = TokenTrainer("gpt2-1hm", vocab=50257, batch_size=8, teacher_entries=64, temperature=2.0, teacher_weight=0.5)
+    loss = trainer.train_step(tokens, teacher=(teacher_ids, teacher_logits))      # [8, 1024] and [8, 1024, 64]
+
+Between the engine's layers and the tokens stand an embedding table and, with the same weights, the projection onto the
+vocabulary: embedding rows go straight into the engine's input, the projection's logits are turned into their gradient in
+place, and the table's gradient is the sum of both ends' (the projection's product assigns it, the embedding's
+adds to it), updated by the engine's Adam.  There is no norm behind the last layer, as in the engine's stack.
+
+Tokens, labels and the teacher's entries are batch-first, the engine's rows sequence-first: the kernels read transposed views.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from .. import parallel as mpu
+from ..models import TransformerConfig
+from ..ops import functional as F
+from .engine import StageEngine
+from .trainer import _DTYPES
+
+
+class TokenTrainer:
+    """``teacher_entries`` > 0: every step brings a teacher's top logits, mixed with the labels' term by ``teacher_weight``.
+    ``embed_scale`` multiplies embedding rows; ``padding_id`` gets no embedding gradient; a label equal to ``ignore_id``
+    counts for nothing.  The loss is the mean over all positions."""
+
+    def __init__(self, model, vocab: int, batch_size: int, *, n_layers: Optional[int] = None, dtype="bf16", lr: float = 1e-4,
+                 activation: str = "gelu", loss_scale: float = 128.0, seed: int = 0, embed_scale: float = 1.0,
+                 padding_id: Optional[int] = None, ignore_id: int = -100, teacher_entries: int = 0, temperature: float = 1.0,
+                 teacher_weight: float = 1.0, use_graph: Optional[bool] = None):
+        topo = mpu.get_topology()
+        if topo.world_size != 1:
+            raise ValueError("TokenTrainer runs on one GPU: one stage, no tensor or data parallelism")
+        cfg = model if isinstance(model, TransformerConfig) else TransformerConfig.from_predefined_model(
+            model, n_devices=1, batch_size=batch_size, n_layers=n_layers, activation=activation)
+        if cfg.batch_size != batch_size:
+            raise ValueError(f"the configuration's batch is {cfg.batch_size}, not {batch_size}")
+        self.config, self.dtype, self.vocab = cfg, _DTYPES[dtype], vocab
+        self.engine = e = StageEngine(cfg, [batch_size], [cfg.seq_len], dtype=self.dtype, loss_scale=loss_scale, lr=lr, seed=seed,
+                                      use_graph=use_graph, merge_slices=True)
+        dev, rows, H = e.device, e.rows, e.H
+        # the projection's tiles want a width of whole 16-byte rows; the columns behind the vocabulary have zero weights, zero
+        # logits and zero gradients
+        width = (vocab + 63) // 64 * 64
+        g = torch.Generator(device=dev).manual_seed(seed + 1)
+        self.master = torch.zeros(width, H, device=dev)
+        self.master[:vocab].normal_(0.0, 0.02, generator=g)
+        self.weight = self.master.to(self.dtype)
+        self.exp_avg, self.exp_avg_sq, self.grad = (torch.zeros_like(self.master) for _ in range(3))
+        self.logits = torch.empty(rows, width, dtype=self.dtype, device=dev)
+        shape = (batch_size, cfg.seq_len)
+        self.tokens, self.labels = (torch.zeros(shape, dtype=torch.int64, device=dev) for _ in range(2))
+        self.teacher = None
+        if teacher_entries:
+            self.teacher = (torch.full((*shape, teacher_entries), -1, dtype=torch.int32, device=dev),
+                            torch.zeros(*shape, teacher_entries, device=dev))
+        self.losses = torch.zeros(rows, device=dev)
+        self.embed_scale, self.padding_id, self.ignore_id = embed_scale, padding_id, ignore_id
+        self.temperature, self.teacher_weight = temperature, teacher_weight
+        self._workspace = torch.empty(F.embedding_bwd_workspace_bytes(rows, vocab, H), dtype=torch.uint8, device=dev)
+        e.ends = self
+
+    # ------------------------------------------------------------------ what the engine calls
+    def begin(self) -> None:
+        F.embedding_fwd(self.tokens.t(), self.weight[:self.vocab], self.engine.X[0], scale=self.embed_scale)
+
+    def _loss_args(self):
+        """The arguments that losses share: without a teacher those of cross entropy."""
+        if self.teacher is None:
+            return (self.labels.t(),), {"ignore_id": self.ignore_id}
+        ids, logits = (t.transpose(0, 1) for t in self.teacher)
+        return (ids, logits, self.labels.t()), {"ignore_id": self.ignore_id, "temperature": self.temperature,
+                                                "teacher_weight": self.teacher_weight}
+
+    def _project(self) -> torch.Tensor:
+        F.gemm(self.engine.X[self.engine.n_layers], self.weight, self.logits)
+        return self.logits[:, :self.vocab]
+
+    def head(self) -> None:
+        e, (args, how) = self.engine, self._loss_args()
+        logits = self._project()
+        loss = F.cross_entropy_fwd_bwd if self.teacher is None else F.distill_fwd_bwd
+        loss(logits, *args, **how, grad_scale=e.loss_scale / e.rows, loss=self.losses, dlogits=logits)
+        F.weight_grad(self.logits, e.X[e.n_layers], self.grad)
+        F.gemm(self.logits, self.weight, e.dY, b_mn=True)
+
+    def finish(self, update: bool) -> None:
+        e = self.engine
+        F.embedding_bwd(self.tokens.t(), e.dA, self.grad[:self.vocab], scale=self.embed_scale, padding_id=self.padding_id,
+                        workspace=self._workspace)
+        if update:
+            F.fused_adam(self.grad, self.master, self.exp_avg, self.exp_avg_sq, self.weight, e.adam_state, lr=e.lr,
+                         grad_scale=1.0 / e.loss_scale)
+
+    # ------------------------------------------------------------------ what a user calls
+    def load(self, tokens: torch.Tensor, labels: Optional[torch.Tensor] = None,
+             teacher: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> None:
+        """Copies a batch ``[batch, seq]``.  Labels that are left out are the following tokens, the last position's none."""
+        if tokens.shape != self.tokens.shape:
+            raise ValueError(f"tokens {tuple(tokens.shape)}, not {tuple(self.tokens.shape)}")
+        if (teacher is None) != (self.teacher is None):
+            raise ValueError("a teacher's entries come with every batch or with none (teacher_entries)")
+        self.tokens.copy_(tokens, non_blocking=True)
+        if labels is None:
+            self.labels[:, :-1].copy_(self.tokens[:, 1:])
+            self.labels[:, -1].fill_(self.ignore_id)
+        else:
+            self.labels.copy_(labels, non_blocking=True)
+        for to, given in zip(self.teacher or (), teacher or ()):
+            if given.shape != to.shape:
+                raise ValueError(f"teacher's entries {tuple(given.shape)}, not {tuple(to.shape)}")
+            to.copy_(given, non_blocking=True)
+
+    def train_step(self, tokens, labels=None, teacher=None) -> float:
+        """One iteration end to end; the mean loss of the weights before it."""
+        self.load(tokens, labels, teacher)
+        self.engine.step()
+        return self._mean()
+
+    def compute_grads(self, tokens, labels=None, teacher=None):
+        """Gradients of the mean loss without an update: the layers' by name, and ``embedding``."""
+        self.load(tokens, labels, teacher)
+        self.engine.compute_grads()
+        grads = self.engine.named_grads()
+        grads["embedding"] = self.grad[:self.vocab] / self.engine.loss_scale
+        return grads
+
+    def evaluate(self, tokens, labels=None, teacher=None) -> float:
+        """The mean loss, forward only."""
+        self.load(tokens, labels, teacher)
+        e, (args, how) = self.engine, self._loss_args()
+        e._refresh_handles()
+        self.begin()
+        e._forward_rows(0, e.rows, e._whole)
+        loss = F.cross_entropy_fwd if self.teacher is None else F.distill_fwd
+        loss(self._project(), *args, **how, loss=self.losses)
+        return self._mean()
+
+    def _mean(self) -> float:
+        mean = float(self.losses.mean())
+        self.engine.check_status()
+        return mean
+
+    def close(self) -> None:
+        self.engine.ends = None
+        self.engine.close()

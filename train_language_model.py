@@ -1,0 +1,68 @@
+#!/usr/bin/env python
+"""Trains a small language model on one GPU on synthetic text, with labels or with a teacher's top logits.
+
+    python train_language_model.py --model test --n-layers 4 --vocab 5000 --batch-size 8 --steps 100
+    python train_language_model.py --model gpt2-1hm --teacher-entries 64 --temperature 2 --teacher-weight 0.5
+
+The text is a random walk: after token ``t`` comes ``(5 t + 7 + d) mod vocab`` with a small ``d`` that is mostly 0.  The
+teacher knows the walk: its top logits are the log-probabilities of the ``d``."""
+import argparse
+import time
+
+import torch
+
+from terapipe_b200.runtime.token_trainer import TokenTrainer
+
+
+def synthetic_batch(vocab, batch, seq, steps_probs, generator):
+    """``[batch, seq + 1]`` tokens of the walk."""
+    d = torch.multinomial(steps_probs, batch * seq, replacement=True, generator=generator).view(batch, seq)
+    out = torch.empty(batch, seq + 1, dtype=torch.int64)
+    out[:, 0] = torch.randint(0, vocab, (batch,), generator=generator)
+    for i in range(seq):
+        out[:, i + 1] = (5 * out[:, i] + 7 + d[:, i]) % vocab
+    return out
+
+
+def main():
+    parser = argparse.ArgumentParser(description="language model training on one GPU")
+    parser.add_argument("--model", default="test")
+    parser.add_argument("--n-layers", type=int, default=None)
+    parser.add_argument("--vocab", type=int, default=5000)
+    parser.add_argument("--batch-size", type=int, default=8)
+    parser.add_argument("--steps", type=int, default=100)
+    parser.add_argument("--lr", type=float, default=1e-3)
+    parser.add_argument("--dtype", choices=("fp16", "bf16"), default="bf16")
+    parser.add_argument("--teacher-entries", type=int, default=0)
+    parser.add_argument("--temperature", type=float, default=1.0)
+    parser.add_argument("--teacher-weight", type=float, default=1.0)
+    parser.add_argument("--seed", type=int, default=0)
+    args = parser.parse_args()
+
+    trainer = TokenTrainer(args.model, args.vocab, args.batch_size, n_layers=args.n_layers, dtype=args.dtype, lr=args.lr, seed=args.seed,
+                           embed_scale=50.0, teacher_entries=args.teacher_entries,
+                           temperature=args.temperature, teacher_weight=args.teacher_weight)
+    seq = trainer.config.seq_len
+    n = max(2, min(args.teacher_entries or 8, args.vocab))
+    probs = torch.softmax(-torch.arange(n, dtype=torch.float32), 0)
+    g = torch.Generator().manual_seed(args.seed)
+    began = time.time()
+    for step in range(args.steps):
+        text = synthetic_batch(args.vocab, args.batch_size, seq, probs, g)
+        tokens, labels = text[:, :-1], text[:, 1:]
+        teacher = None
+        if args.teacher_entries:
+            ids = (5 * tokens[..., None] + 7 + torch.arange(n)) % args.vocab
+            ids = torch.cat([ids, ids.new_full((*tokens.shape, args.teacher_entries - n), -1)], -1)
+            logits = torch.zeros(ids.shape)
+            logits[..., :n] = probs.log()
+            teacher = (ids, logits)
+        loss = trainer.train_step(tokens, labels, teacher)
+        if step % 10 == 0 or step == args.steps - 1:
+            print(f"step {step:4d}  loss {loss:.4f}", flush=True)
+    print(f"{args.steps * args.batch_size * seq / (time.time() - began):.0f} tokens/s")
+    trainer.close()
+
+
+if __name__ == "__main__":
+    main()
