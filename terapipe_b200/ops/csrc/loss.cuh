@@ -32,7 +32,7 @@ struct LossArgs {
   int top, tid64, tlog_dtype;
   float temperature, weight;     // weight = a
   float* loss;                   // [rows]
-  float* stats;                  // [rows][4]: largest logit (0 where all are -inf), sum of exp(z - largest), of exp((z - largest) / T)
+  float* stats;                  // [rows][8], see store_loss
   void* dlogits;
   long long ldd;
   const float* grad_loss;        // [rows], stride ldg; null: 1
@@ -279,18 +279,23 @@ __device__ __forceinline__ void send_part(const PartOfRow& p, uint32_t cluster_a
                ::"r"(cluster_addr + 16), "f"(p.mass), "f"(p.zy), "f"(p.own), "f"(p.pad), "r"(cluster_bar) : "memory");
 }
 
-// t_sum: sum of exp((t - t_max) / T) over the entries; entropy: the same weighted with (t - t_max) / T.
-__device__ __forceinline__ void store_loss(const LossArgs& a, int row, const WholeRow& w, bool label, bool teach, float t_sum,
+// t_max: largest of the teacher's logits (0 where there is none), t_sum: sum of exp((t - t_max) / T) over the entries, entropy: the same
+// weighted with (t - t_max) / T.  stats: largest logit (0 where all are -inf), sums of exp(z - largest) and of
+// exp((z - largest) / T), t_max, t_sum.
+__device__ __forceinline__ void store_loss(const LossArgs& a, int row, const WholeRow& w, bool label, bool teach, float t_max, float t_sum,
                                            float entropy) {
   float loss = 0.0f;
   if (w.s1 != 0.0f) {
     if (label) loss = (1.0f - a.weight) * (__logf(w.s1) - w.zy);
     if (teach)
-      loss += a.weight * a.temperature * a.temperature *
-              ((entropy - w.dot / a.temperature) / t_sum - __logf(t_sum) + __logf(w.st));
+      loss += a.weight * a.temperature * a.temperature * ((entropy - w.dot / a.temperature) / t_sum - __logf(t_sum) + __logf(w.st));
   }
   a.loss[row] = loss;
-  if (a.stats) *reinterpret_cast<float4*>(a.stats + 4ll * row) = make_float4(w.m, w.s1, w.st, 0.0f);
+  if (a.stats) {
+    float4* p = reinterpret_cast<float4*>(a.stats + 8ll * row);
+    p[0] = make_float4(w.m, w.s1, w.st, t_max);
+    p[1] = make_float4(t_sum, 0.0f, 0.0f, 0.0f);
+  }
 }
 
 // The gradient's element of entry k, by the first of the entries with its id.  e1, et: exponentials of its logit, g1: the label's
@@ -352,7 +357,7 @@ struct alignas(16) RowKnown {
 };
 // What is known of a row before its sums: its label and entries.
 struct RowTerms {
-  float g, zy, t_sum, entropy;      // the row's factor; z_y if the label is in this part; sums over all entries
+  float g, zy, t_max, t_sum, entropy;      // the row's factor; z_y if the label is in this part; of all entries
   int label, listed;                // -1: no label; entries listed
   bool teach, own, twice;           // the row has the teacher's term; the label is in this part; an id occurs twice in it
 };
@@ -571,7 +576,7 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
         whole.dot = warp_add<8>(v.x);
         whole.zy = warp_add<8>(v.y);
       }
-      if (lane == 0) store_loss(a, row, whole, t_last.label >= 0, t_last.teach, t_last.t_sum, t_last.entropy);
+      if (lane == 0) store_loss(a, row, whole, t_last.label >= 0, t_last.teach, t_last.t_max, t_last.t_sum, t_last.entropy);
       return true;
     };
     int n = 0;      // rows done
@@ -675,7 +680,7 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
       float* list_p = list_p_all + (n & 3) * a.top;
       float* list_z = list_z_all + (n & 3) * a.top;
       int* list_id = list_id_all + (n & 3) * a.top;
-      RowTerms now{raw_g, 0.0f, 0.0f, 0.0f, raw_label.get(a), 0, false, false, false};
+      RowTerms now{raw_g, 0.0f, 0.0f, 0.0f, 0.0f, raw_label.get(a), 0, false, false, false};
       float t_max = -INFINITY;
       for (int k0 = 0; k0 < a.top; k0 += 32 * kAhead) {
         if (k0 > 0) load_entries<kAhead>(a, row, k0 + lane, raw_entry);
@@ -691,7 +696,7 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
       if (row + stride < a.rows) load_raw(row + stride);
       if (teacher) {
         t_max = warp_max(t_max);
-        if (t_max == -INFINITY) t_max = 0.0f;
+        now.t_max = t_max = t_max == -INFINITY ? 0.0f : t_max;
 #pragma unroll 1
         for (int k0 = 0; k0 < a.top; k0 += 32) {
           const int k = k0 + lane, id = k < a.top ? top_id[k] : -1, at = place(r, id);
@@ -750,9 +755,8 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
 }
 
 // ------------------------------------------------------------------ rows read twice
-// The gradient from a forward pass's statistics (MODE 2), and rows that a cluster cannot hold (1 and 3: the second read is
-// served by L2 where it can).  A CTA per part of a row; the parts of a row form a cluster where their sums have to be joined.
-template <typename T, int SOFT, int MODE>
+// Rows that a cluster cannot hold: the second read is served by L2 where it can.  A CTA per part of a row, a cluster per row.
+template <typename T, int SOFT, bool WRITE>
 __global__ void __launch_bounds__(512, 2)
 loss_stream_kernel(const LossArgs a, int parts, int per) {
   constexpr bool DUAL = SOFT != 0, POWER = SOFT == 2;
@@ -793,7 +797,7 @@ loss_stream_kernel(const LossArgs a, int parts, int per) {
     top_z[k] = in_part(id) ? Elem<T>::to_f(r.row[id]) : 0.0f;
     t_max = fmaxf(t_max, t);
   }
-  if (MODE & kLossFwd) {
+  {
     for (int g = g0 + tid; g < g1; g += kThreads * kAhead) {
       uint4 u[kAhead];
       GranuleMax<T> largest;
@@ -840,10 +844,8 @@ loss_stream_kernel(const LossArgs a, int parts, int per) {
   t_max = warp_max(red_max[1][lane % kWarps]);
   if (t_max == -INFINITY) t_max = 0.0f;
   const float shift = m == -INFINITY ? 0.0f : m;
-  if (MODE & kLossFwd) {
-    s1 *= Exponent{k1, shift}.factor(m_mine);
-    if (DUAL) st *= Exponent{kt, shift}.factor(m_mine);
-  }
+  s1 *= Exponent{k1, shift}.factor(m_mine);
+  if (DUAL) st *= Exponent{kt, shift}.factor(m_mine);
   float t_part = 0.0f, entropy = 0.0f, dot = 0.0f, mass = 0.0f;
   for (int k = tid; k < a.top; k += kThreads) {
     const int id = top_id[k];
@@ -856,10 +858,8 @@ loss_stream_kernel(const LossArgs a, int parts, int per) {
     dot += p * (top_z[k] - shift);
     mass += p;
   }
-  if (MODE & kLossFwd) {
-    s1 = warp_add(s1);
-    if (DUAL) st = warp_add(st);
-  }
+  s1 = warp_add(s1);
+  if (DUAL) st = warp_add(st);
   if (teacher) {
     t_part = warp_add(t_part);
     entropy = warp_add(entropy);
@@ -878,25 +878,20 @@ loss_stream_kernel(const LossArgs a, int parts, int per) {
   const float t_sum = teacher ? add_up<kWarps>(red_sum[2]) : 0.0f;
   const bool teach = a.weight != 0.0f && t_sum != 0.0f;
   WholeRow w;
-  if (MODE & kLossFwd) {
-    PartOfRow p{m, add_up<kWarps>(red_sum[0]), DUAL ? add_up<kWarps>(red_sum[1]) : 0.0f, add_up<kWarps>(red_sum[4]),
-                add_up<kWarps>(red_sum[5]), own ? zy - shift : 0.0f, own ? 1.0f : 0.0f, 0};
-    if (parts > 1) {
-      if (tid == 0) part = p;
-      cluster_sync_all();
-      if (lane < parts) p = load_part(mapa_u32(smem_u32(&part), lane));
-      w = join_parts<DUAL>(p, parts, k1, kt, teacher);
-    } else {
-      w = WholeRow{shift, p.s1, DUAL ? p.st : p.s1, p.dot, p.zy};
-    }
-    entropy = add_up<kWarps>(red_sum[3]);
-    if (rank == 0 && tid == 0) store_loss(a, row, w, label >= 0, teach, t_sum, entropy);
-    if (parts > 1) cluster_sync_all();      // nobody leaves while its part may still be read
+  PartOfRow p{m, add_up<kWarps>(red_sum[0]), DUAL ? add_up<kWarps>(red_sum[1]) : 0.0f, add_up<kWarps>(red_sum[4]),
+              add_up<kWarps>(red_sum[5]), own ? zy - shift : 0.0f, own ? 1.0f : 0.0f, 0};
+  if (parts > 1) {
+    if (tid == 0) part = p;
+    cluster_sync_all();
+    if (lane < parts) p = load_part(mapa_u32(smem_u32(&part), lane));
+    w = join_parts<DUAL>(p, parts, k1, kt, teacher);
   } else {
-    const float4 v = *reinterpret_cast<const float4*>(a.stats + 4ll * row);
-    w = WholeRow{v.x, v.y, v.z, 0.0f, 0.0f};
+    w = WholeRow{shift, p.s1, DUAL ? p.st : p.s1, p.dot, p.zy};
   }
-  if (!(MODE & kLossBwd)) return;
+  entropy = add_up<kWarps>(red_sum[3]);
+  if (rank == 0 && tid == 0) store_loss(a, row, w, label >= 0, teach, t_max, t_sum, entropy);
+  if (parts > 1) cluster_sync_all();      // nobody leaves while its part may still be read
+  if (!WRITE) return;
   const bool zero = !(teach || label >= 0) || w.s1 == 0.0f;
   const RowFactors f(a, a.grad_loss ? a.grad_loss[row * a.ldg] : 1.0f, label >= 0, teach);
   const Exponent x1{k1, w.m}, xt{kt, w.m};
@@ -935,6 +930,108 @@ loss_stream_kernel(const LossArgs a, int parts, int per) {
     if (in_part(top_id[k]))
       store_entry<T, DUAL>(out, top_id[k], k, exp2_approx(x1(top_z[k])), DUAL ? exp2_approx(xt(top_z[k])) : 0.0f, top_id, top_p, a.top,
                            true, c1, ct, f.g1, f.gt / t_sum, label);
+}
+
+// ------------------------------------------------------------------ the gradient from a forward pass's statistics
+// A CTA per part of a row, four granules a thread.  Bound by the bytes; what a row needs besides is on its way together with its
+// logits.  (With the sums of the forward kernel's kind over the teacher's entries before the logits were asked for, 2045 rows of
+// 32000 fp32 logits took 207 us, FAST this way; of 16384 rows of 2000, 512 threads each, 164 and SMALL.)
+template <typename T, int SOFT, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
+loss_bwd_kernel(const LossArgs a, int parts, int table) {
+  constexpr bool DUAL = SOFT != 0, POWER = SOFT == 2;
+  constexpr int N = Granule<T>::N, kNG = 4, kPer = THREADS * kNG;
+  extern __shared__ __align__(16) uint4 loss_smem[];
+  float* top_p = reinterpret_cast<float*>(loss_smem);      // [top] p
+  float* top_z = top_p + a.top;                            // [top] z
+  int* top_id = reinterpret_cast<int*>(top_z + a.top);     // [top] -1 outside this part
+  int* ids = top_id + a.top;                               // [table] hash table of id + 1
+  __shared__ int twice;
+  const int tid = threadIdx.x, rank = blockIdx.x % parts, row = blockIdx.x / parts;
+  const float inv_t = 1.0f / a.temperature, kt = inv_t * kLog2e;
+  const float k1 = DUAL || a.weight == 0.0f ? kLog2e : kt;
+  const int power = static_cast<int>(a.temperature);
+  pdl_wait();
+  const RowPieces<T> r(static_cast<const T*>(a.logits) + row * a.ld, a.V);
+  const int g0 = rank * kPer, cnt = min(r.count - g0, kPer);
+  uint4 u[kNG];
+#pragma unroll
+  for (int k = 0; k < kNG; ++k) {
+    const int gl = tid + k * THREADS;
+    if (gl < cnt && !r.edge(g0 + gl)) u[k] = __ldcs(reinterpret_cast<const uint4*>(r.row - r.lead) + g0 + gl);
+  }
+  RawLabel raw_label{};
+  raw_label.load(a, row);
+  const float4 s0 = reinterpret_cast<const float4*>(a.stats)[2 * row];
+  const float t_max = s0.w, t_sum = a.stats[8ll * row + 4], g = a.grad_loss ? a.grad_loss[row * a.ldg] : 1.0f;
+#pragma unroll
+  for (int k = 0; k < kNG; ++k) {
+    const int gl = tid + k * THREADS;
+    if (gl < cnt && r.edge(g0 + gl)) u[k] = r.load_edge(g0 + gl);
+  }
+  const int label = raw_label.get(a);
+  auto in_part = [&](int id) {
+    const int at = id + r.lead - g0 * N;
+    return id >= 0 && at >= 0 && at < kPer * N;
+  };
+  const bool own = in_part(label);
+  const float zy = own ? Elem<T>::to_f(r.row[label]) : 0.0f;
+  if (a.top > 0) {
+    if (tid == 0) twice = 0;
+    for (int i = tid; i < table; i += THREADS) ids[i] = 0;
+    __syncthreads();
+    for (int k = tid; k < a.top; k += THREADS) {
+      RawEntry e[1];
+      load_entries<1>(a, row, k, e);
+      const int id = e[0].id(a), at = in_part(id) ? id : -1;
+      top_id[k] = at;
+      if (at < 0) continue;
+      top_p[k] = exp2_approx((e[0].logit(a) - t_max) * kt);
+      top_z[k] = Elem<T>::to_f(r.row[id]);
+      int slot = static_cast<int>(id * 0x9e3779b1u >> 16) & (table - 1);
+      while (true) {      // (at most half of the slots are ever taken)
+        const int was = atomicCAS(&ids[slot], 0, id + 1);
+        if (was == id + 1) twice = 1;
+        if (was == 0 || was == id + 1) break;
+        slot = (slot + 1) & (table - 1);
+      }
+    }
+  }
+  __syncthreads();      // the label's and every entry's logit has been read before the row is written
+  const float m = s0.x, s1 = s0.y, st = s0.z;
+  const bool teach = a.weight != 0.0f && t_sum != 0.0f, zero = !(teach || label >= 0) || s1 == 0.0f;
+  const RowFactors f(a, g, label >= 0, teach);
+  const Exponent x1{k1, m}, xt{kt, m};
+  const float c1 = (DUAL ? f.g1 : f.g1 + f.gt) * (1.0f / s1), ct = DUAL ? f.gt * (1.0f / st) : 0.0f;
+  T* out = static_cast<T*>(a.dlogits) + row * a.ldd;
+  const bool wide = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(r.row)) & 15) == 0;
+#pragma unroll
+  for (int k = 0; k < kNG; ++k) {
+    const int gl = tid + k * THREADS;
+    if (gl >= cnt) continue;
+    float o[N] = {};
+    if (!zero) {
+      float e[N], e2[N];
+      if (DUAL) granule_exp<T>(u[k], xt, e2);
+      if (!POWER) granule_exp<T>(u[k], x1, e);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float v1 = POWER ? raise2(make_float2(e2[j], e2[j]), power).x : e[j];
+        o[j] = DUAL ? fmaf(ct, e2[j], c1 * v1) : c1 * v1;
+      }
+    }
+    r.store(out, g0 + gl, o, wide && !r.edge(g0 + gl));
+  }
+  if (zero || !(own || teach)) return;      // (the same for all threads)
+  __syncthreads();      // the label's and the entries' elements come after the row's
+  if (tid == 0 && own)
+    out[label] = Elem<T>::from_f((c1 * exp2_approx(x1(zy)) - f.g1) + (DUAL ? ct * exp2_approx(xt(zy)) : 0.0f));
+  if (!teach) return;
+  __syncthreads();
+  for (int k = tid; k < a.top; k += THREADS)
+    if (top_id[k] >= 0)
+      store_entry<T, DUAL>(out, top_id[k], k, exp2_approx(x1(top_z[k])), DUAL ? exp2_approx(xt(top_z[k])) : 0.0f, top_id, top_p, a.top,
+                           twice, c1, ct, f.g1, f.gt / t_sum, label);
 }
 
 // ------------------------------------------------------------------ launches
@@ -978,11 +1075,20 @@ static int loss_rows_launch(const LossArgs& a, int parts, int per, cudaStream_t 
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
 
-template <typename T, int SOFT, int MODE> static int loss_stream_launch(const LossArgs& a, int parts, int per, cudaStream_t s) {
+template <typename T, int SOFT, bool WRITE> static int loss_stream_launch(const LossArgs& a, int parts, int per, cudaStream_t s) {
   const long long grid = static_cast<long long>(a.rows) * parts;
   if (grid > 0x7fffffffll) return kErrTooLarge;
-  launch_pdl(loss_stream_kernel<T, SOFT, MODE>, dim3(static_cast<unsigned>(grid)), dim3(512), static_cast<size_t>(a.top) * 12, s,
-             MODE & kLossFwd ? parts : 1, a, parts, per);
+  launch_pdl(loss_stream_kernel<T, SOFT, WRITE>, dim3(static_cast<unsigned>(grid)), dim3(512), static_cast<size_t>(a.top) * 12, s, parts, a,
+             parts, per);
+  return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
+}
+
+template <typename T, int SOFT, int THREADS> static int loss_bwd_launch(const LossArgs& a, int parts, cudaStream_t s) {
+  const long long grid = static_cast<long long>(a.rows) * parts;
+  if (grid > 0x7fffffffll) return kErrTooLarge;
+  const int table = a.top > 0 ? loss_table_size(a.top) : 0;
+  launch_pdl(loss_bwd_kernel<T, SOFT, THREADS>, dim3(static_cast<unsigned>(grid)), dim3(THREADS), 12ull * a.top + 4ull * table, s, 1, a, parts,
+             table);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
 
@@ -996,8 +1102,11 @@ static int loss_rows_fit(const LossArgs& a, int parts, int per, cudaStream_t s) 
   return loss_rows_launch<T, SOFT, THREADS, NG, WRITE>(a, parts, per, s);
 }
 
+#ifndef PMOST
+#define PMOST 4
+#endif
 template <typename T, int SOFT, bool WRITE> static int loss_choose(const LossArgs& a, cudaStream_t s) {
-  constexpr int N = Granule<T>::N, kMost = SOFT == 1 ? 4 : 8;      // granules a thread: registers for their exponentials
+  constexpr int N = Granule<T>::N, kMost = SOFT == 1 ? 4 : SOFT == 2 ? PMOST : 8;      // granules a thread: registers for their exponentials
   // granules of the longest row: rows on different offsets from a 16-byte boundary may need one more
   const bool same = a.rows == 1 || a.ld * static_cast<long long>(sizeof(T)) % 16 == 0;
   const long long lead = same ? (reinterpret_cast<uintptr_t>(a.logits) & 15) / sizeof(T) : N - 1;
@@ -1009,15 +1118,15 @@ template <typename T, int SOFT, bool WRITE> static int loss_choose(const LossArg
   const int per = static_cast<int>((granules + parts - 1) / parts);
   if (per <= 256 * kMost) return loss_rows_fit<T, SOFT, 256, kMost, WRITE>(a, parts, per, s);
   if (per <= 512 * kMost) return loss_rows_fit<T, SOFT, 512, kMost, WRITE>(a, parts, per, s);
-  return loss_stream_launch<T, SOFT, kLossFwd | (WRITE ? kLossBwd : 0)>(a, parts, per, s);
+  return loss_stream_launch<T, SOFT, WRITE>(a, parts, per, s);
 }
 
 template <typename T, int SOFT> static int loss_mode(const LossArgs& a, int mode, cudaStream_t s) {
   if (mode == kLossFwd) return loss_choose<T, SOFT, false>(a, s);
   if (mode == (kLossFwd | kLossBwd)) return loss_choose<T, SOFT, true>(a, s);
-  const int per = 2048;
   const long long granules = (a.V + 2ll * Granule<T>::N - 2) / Granule<T>::N;
-  return loss_stream_launch<T, SOFT, kLossBwd>(a, static_cast<int>(granules > per ? (granules + per - 1) / per : 1), per, s);
+  if (granules <= 512) return loss_bwd_launch<T, SOFT, 128>(a, 1, s);
+  return loss_bwd_launch<T, SOFT, 256>(a, static_cast<int>((granules + 1023) / 1024), s);
 }
 
 template <typename T> static int loss_launch(const LossArgs& a, int mode, cudaStream_t s) {

@@ -428,9 +428,10 @@ def _loss(mode, logits, teacher, labels, temperature, teacher_weight, ignore_id,
         elif loss.dtype != torch.float32 or loss.numel() != n or not loss.is_contiguous():
             raise KernelError(f"loss is float32 [{n}], contiguous")
     if mode == 1 and stats is None:
-        stats = torch.empty(n, 4, dtype=torch.float32, device=logits.device)
-    elif stats is not None and (stats.dtype != torch.float32 or stats.numel() != 4 * n or not stats.is_contiguous()):
-        raise KernelError(f"stats is float32 [{n}, 4], contiguous")
+        stats = torch.empty(n, 8, dtype=torch.float32, device=logits.device)
+    elif stats is not None and (stats.dtype != torch.float32 or stats.numel() != 8 * n or not stats.is_contiguous()
+                                or stats.data_ptr() % 16):
+        raise KernelError(f"stats is float32 [{n}, 8], contiguous on a 16-byte boundary")
     ldd = ldg = 0
     if mode & 2:
         if dlogits is None:
@@ -462,7 +463,7 @@ def _loss(mode, logits, teacher, labels, temperature, teacher_weight, ignore_id,
 def distill_fwd(logits, teacher_ids, teacher_logits, labels=None, *, temperature: float = 1.0, teacher_weight: float = 1.0,
                 ignore_id: int = -100, loss=None, stats=None):
     """Loss of every row of ``logits`` against a teacher's top logits; returns ``(loss, stats)``, fp32 ``[rows]`` and the
-    ``[rows, 4]`` that :func:`distill_bwd` needs.
+    ``[rows, 8]`` that :func:`distill_bwd` needs.
 
     ``loss = (1 - teacher_weight) * (logsumexp(z) - z[label]) + teacher_weight * T^2 * sum_k p_k (log p_k - log q[id_k])``
     with ``p`` the softmax of the row's teacher logits divided by the temperature ``T`` and ``q`` that of ``z / T`` over the
