@@ -193,17 +193,15 @@ __device__ __forceinline__ void granule_exp(const uint4& u, const Exponent& x, f
     e[j + 1] = exp2_approx(d.y);
   }
 }
-// x^n, n = 2, 3 or 4: with a temperature of n the exponential of z - shift is that power of the exponential of (z - shift) / n.
-__device__ __forceinline__ float2 raise2(float2 x, int n) {
-  float2 r = mul2(x, x);
-  if (n == 3) r = mul2(r, x);
-  if (n == 4) r = mul2(r, r);
-  return r;
+// x^P, P = 2 or 4: with a temperature of P the exponential of z - shift is that power of the exponential of (z - shift) / P.
+template <int P> __device__ __forceinline__ float2 raise2(float2 x) {
+  const float2 r = mul2(x, x);
+  return P == 4 ? mul2(r, r) : r;
 }
-template <int N> __device__ __forceinline__ float sum_of_powers(const float (&e)[N], int n) {
-  float2 s = raise2(make_float2(e[0], e[1]), n);
+template <int P, int N> __device__ __forceinline__ float sum_of_powers(const float (&e)[N]) {
+  float2 s = raise2<P>(make_float2(e[0], e[1]));
 #pragma unroll
-  for (int j = 2; j < N; j += 2) s = add2(s, raise2(make_float2(e[j], e[j + 1]), n));
+  for (int j = 2; j < N; j += 2) s = add2(s, raise2<P>(make_float2(e[j], e[j + 1])));
   return s.x + s.y;
 }
 template <int N> __device__ __forceinline__ float sum_of(const float (&e)[N]) {
@@ -396,7 +394,7 @@ struct PartGeom {
 template <typename T, int SOFT, int THREADS, int NG, bool WRITE>
 __global__ void __launch_bounds__(THREADS + 64, loss_ctas_per_sm(THREADS, (WRITE ? NG : 1) * Granule<T>::N * (SOFT == 1 ? 2 : 1)))
 loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
-  constexpr bool DUAL = SOFT != 0, POWER = SOFT == 2;
+  constexpr bool DUAL = SOFT != 0, POWER = SOFT >= 2;
   constexpr int N = Granule<T>::N, kWarps = THREADS / 32, kSlots = THREADS * NG, kKept = WRITE ? NG : 1, kMaxParts = 8, kAhead = 4;
   extern __shared__ __align__(16) uint4 loss_smem[];
   uint4* raw = loss_smem;                                          // [2][kSlots]
@@ -416,7 +414,6 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
   const int rank = parts > 1 ? cluster_ctarank() : 0;
   const int stride = gridDim.x / parts, g0 = rank * per, senders = parts * kWarps;
   const bool teacher = a.top > 0;
-  const int power = static_cast<int>(a.temperature);
   const float inv_t = 1.0f / a.temperature, kt = inv_t * kLog2e;
   // the one exponential's exponent without DUAL: z, or with a teacher alone z / T
   const float k1 = DUAL || a.weight == 0.0f ? kLog2e : kt;
@@ -466,7 +463,7 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
           st += sum_of<N>(et[kept]);
         }
         if (POWER) {
-          s1 += sum_of_powers<N>(et[kept], power);
+          s1 += sum_of_powers<SOFT, N>(et[kept]);
         } else {
           granule_exp<T>(u, x1, e1[kept]);
           s1 += sum_of<N>(e1[kept]);
@@ -504,7 +501,7 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
 #pragma unroll
           for (int j = 0; j < N; j += 2) {
             const float2 d2 = DUAL ? make_float2(et[k][j], et[k][j + 1]) : make_float2(0.0f, 0.0f);
-            float2 d = mul2(POWER ? raise2(d2, power) : make_float2(e1[POWER ? 0 : k][j], e1[POWER ? 0 : k][j + 1]), dup2(c1));
+            float2 d = mul2(POWER ? raise2<SOFT>(d2) : make_float2(e1[POWER ? 0 : k][j], e1[POWER ? 0 : k][j + 1]), dup2(c1));
             if (DUAL) d = fma2(d2, dup2(ct), d);
             v[j] = d.x;
             v[j + 1] = d.y;
@@ -520,7 +517,7 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
             float v[N];
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-              const float vt = DUAL ? et[k][j] : 0.0f, v1 = POWER ? raise2(make_float2(vt, vt), power).x : e1[POWER ? 0 : k][j];
+              const float vt = DUAL ? et[k][j] : 0.0f, v1 = POWER ? raise2<SOFT>(make_float2(vt, vt)).x : e1[POWER ? 0 : k][j];
               v[j] = DUAL ? fmaf(ct, vt, c1 * v1) : c1 * v1;
             }
             r.store(out, g0 + gl, v, false);
@@ -759,7 +756,7 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
 template <typename T, int SOFT, bool WRITE>
 __global__ void __launch_bounds__(512, 2)
 loss_stream_kernel(const LossArgs a, int parts, int per) {
-  constexpr bool DUAL = SOFT != 0, POWER = SOFT == 2;
+  constexpr bool DUAL = SOFT != 0, POWER = SOFT >= 2;
   constexpr int N = Granule<T>::N, kWarps = 16, kThreads = 512, kAhead = 4;
   extern __shared__ __align__(16) uint4 loss_smem[];
   float* top_p = reinterpret_cast<float*>(loss_smem);
@@ -772,7 +769,6 @@ loss_stream_kernel(const LossArgs a, int parts, int per) {
   const float inv_t = 1.0f / a.temperature, kt = inv_t * kLog2e;
   const float k1 = DUAL || a.weight == 0.0f ? kLog2e : kt;
   const bool teacher = a.top > 0;
-  const int power = static_cast<int>(a.temperature);
   pdl_wait();
   const RowPieces<T> r(static_cast<const T*>(a.logits) + row * a.ld, a.V);
   const int g0 = static_cast<int>(min(static_cast<long long>(rank) * per, static_cast<long long>(r.count)));
@@ -824,7 +820,7 @@ loss_stream_kernel(const LossArgs a, int parts, int per) {
           st += sum_of<N>(e2);
         }
         if (POWER) {
-          s1 += sum_of_powers<N>(e2, power);
+          s1 += sum_of_powers<SOFT, N>(e2);
         } else {
           granule_exp<T>(u[k], x1, e);
           s1 += sum_of<N>(e);
@@ -913,7 +909,7 @@ loss_stream_kernel(const LossArgs a, int parts, int per) {
         if (!POWER) granule_exp<T>(u[k], x1, e);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          const float v1 = POWER ? raise2(make_float2(e2[j], e2[j]), power).x : e[j];
+          const float v1 = POWER ? raise2<SOFT>(make_float2(e2[j], e2[j])).x : e[j];
           o[j] = DUAL ? fmaf(ct, e2[j], c1 * v1) : c1 * v1;
         }
       }
@@ -939,7 +935,7 @@ loss_stream_kernel(const LossArgs a, int parts, int per) {
 template <typename T, int SOFT, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 loss_bwd_kernel(const LossArgs a, int parts, int table) {
-  constexpr bool DUAL = SOFT != 0, POWER = SOFT == 2;
+  constexpr bool DUAL = SOFT != 0, POWER = SOFT >= 2;
   constexpr int N = Granule<T>::N, kNG = 4, kPer = THREADS * kNG;
   extern __shared__ __align__(16) uint4 loss_smem[];
   float* top_p = reinterpret_cast<float*>(loss_smem);      // [top] p
@@ -950,7 +946,6 @@ loss_bwd_kernel(const LossArgs a, int parts, int table) {
   const int tid = threadIdx.x, rank = blockIdx.x % parts, row = blockIdx.x / parts;
   const float inv_t = 1.0f / a.temperature, kt = inv_t * kLog2e;
   const float k1 = DUAL || a.weight == 0.0f ? kLog2e : kt;
-  const int power = static_cast<int>(a.temperature);
   pdl_wait();
   const RowPieces<T> r(static_cast<const T*>(a.logits) + row * a.ld, a.V);
   const int g0 = rank * kPer, cnt = min(r.count - g0, kPer);
@@ -1016,7 +1011,7 @@ loss_bwd_kernel(const LossArgs a, int parts, int table) {
       if (!POWER) granule_exp<T>(u[k], x1, e);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const float v1 = POWER ? raise2(make_float2(e2[j], e2[j]), power).x : e[j];
+        const float v1 = POWER ? raise2<SOFT>(make_float2(e2[j], e2[j])).x : e[j];
         o[j] = DUAL ? fmaf(ct, e2[j], c1 * v1) : c1 * v1;
       }
     }
@@ -1094,35 +1089,33 @@ template <typename T, int SOFT, int THREADS> static int loss_bwd_launch(const Lo
 
 // The kernel for `per` granules a part at THREADS threads: the parts of a row differ by at most 8 granules (its last part, and the
 // granule more that an offset from a 16-byte boundary needs), so that all but the last two granules a thread are full.
-template <typename T, int SOFT, int THREADS, int NG, bool WRITE>
+// LEAST: the smallest NG that a caller has use for.
+template <typename T, int SOFT, int THREADS, int NG, int LEAST, bool WRITE>
 static int loss_rows_fit(const LossArgs& a, int parts, int per, cudaStream_t s) {
-  if constexpr (NG > 1) {
-    if (per <= THREADS * (NG - 1)) return loss_rows_fit<T, SOFT, THREADS, NG - 1, WRITE>(a, parts, per, s);
+  if constexpr (NG > LEAST) {
+    if (per <= THREADS * (NG - 1)) return loss_rows_fit<T, SOFT, THREADS, NG - 1, LEAST, WRITE>(a, parts, per, s);
   }
   return loss_rows_launch<T, SOFT, THREADS, NG, WRITE>(a, parts, per, s);
 }
 
-#ifndef PMOST
-#define PMOST 4
-#endif
 template <typename T, int SOFT, bool WRITE> static int loss_choose(const LossArgs& a, cudaStream_t s) {
-  constexpr int N = Granule<T>::N, kMost = SOFT == 1 ? 4 : SOFT == 2 ? PMOST : 8;      // granules a thread: registers for their exponentials
+  constexpr int N = Granule<T>::N, kMost = WRITE && SOFT == 1 ? 4 : 8;      // granules a thread: registers for their exponentials
   // granules of the longest row: rows on different offsets from a 16-byte boundary may need one more
   const bool same = a.rows == 1 || a.ld * static_cast<long long>(sizeof(T)) % 16 == 0;
   const long long lead = same ? (reinterpret_cast<uintptr_t>(a.logits) & 15) / sizeof(T) : N - 1;
   const long long granules = (a.V + lead + N - 1) / N;
-  if (granules <= 128 * 4) return loss_rows_fit<T, SOFT, 128, 4, WRITE>(a, 1, static_cast<int>(granules), s);
+  if (granules <= 128 * 4) return loss_rows_fit<T, SOFT, 128, 4, 1, WRITE>(a, 1, static_cast<int>(granules), s);
   int parts = 1;
   while (parts < 8 && granules > parts * 256ll * kMost) parts *= 2;
   while (parts < 8 && a.rows * parts * 2ll <= num_sms() && granules > parts * 512ll) parts *= 2;
   const int per = static_cast<int>((granules + parts - 1) / parts);
-  if (per <= 256 * kMost) return loss_rows_fit<T, SOFT, 256, kMost, WRITE>(a, parts, per, s);
-  if (per <= 512 * kMost) return loss_rows_fit<T, SOFT, 512, kMost, WRITE>(a, parts, per, s);
+  if (per <= 256 * kMost) return loss_rows_fit<T, SOFT, 256, kMost, 1, WRITE>(a, parts, per, s);
+  if (per <= 512 * kMost) return loss_rows_fit<T, SOFT, 512, kMost, kMost / 2 + 1, WRITE>(a, parts, per, s);
   return loss_stream_launch<T, SOFT, WRITE>(a, parts, per, s);
 }
 
 template <typename T, int SOFT> static int loss_mode(const LossArgs& a, int mode, cudaStream_t s) {
-  if (mode == kLossFwd) return loss_choose<T, SOFT, false>(a, s);
+  if (mode == kLossFwd) return loss_choose<T, SOFT != 0, false>(a, s);      // (nothing is kept: a power saves nothing)
   if (mode == (kLossFwd | kLossBwd)) return loss_choose<T, SOFT, true>(a, s);
   const long long granules = (a.V + 2ll * Granule<T>::N - 2) / Granule<T>::N;
   if (granules <= 512) return loss_bwd_launch<T, SOFT, 128>(a, 1, s);
@@ -1131,7 +1124,8 @@ template <typename T, int SOFT> static int loss_mode(const LossArgs& a, int mode
 
 template <typename T> static int loss_launch(const LossArgs& a, int mode, cudaStream_t s) {
   if (a.weight > 0.0f && a.weight < 1.0f && a.top > 0 && a.labels && a.temperature != 1.0f) {
-    if (a.temperature == 2.0f || a.temperature == 3.0f || a.temperature == 4.0f) return loss_mode<T, 2>(a, mode, s);
+    if (a.temperature == 2.0f) return loss_mode<T, 2>(a, mode, s);
+    if (a.temperature == 4.0f) return loss_mode<T, 4>(a, mode, s);
     return loss_mode<T, 1>(a, mode, s);
   }
   return loss_mode<T, 0>(a, mode, s);
