@@ -3,26 +3,51 @@
 
 using namespace tp;
 
-// mode: 1 loss and stats, 2 gradient from stats, 3 loss and gradient.  dtype, tlog_dtype: 0 fp16, 1 bf16, 2 fp32.  Outer
-// index i of an array lies at (i / cols) * s0 + (i % cols) * s1.  dlogits may be logits.
-extern "C" int tp_loss(int mode, int dtype, const void* logits, long long ld, int rows, int V, const void* labels,
-                       int labels64, int label_cols, long long label_s0, long long label_s1, long long ignore,
-                       const void* tid, int tid64, int tid_cols, long long tid_s0, long long tid_s1, const void* tlog,
-                       int tlog_dtype, int tlog_cols, long long tlog_s0, long long tlog_s1, int top, float temperature,
-                       float weight, float* loss, float* stats, void* dlogits, long long ldd, const float* grad_loss,
-                       long long ldg, float grad_scale, int* status, void* stream) {
-  if (mode < 1 || mode > 3 || dtype < 0 || dtype > 2 || tlog_dtype < 0 || tlog_dtype > 2 || rows < 0 || V < 0 || top < 0 ||
-      label_cols < 1 || tid_cols < 1 || tlog_cols < 1 || !(temperature >= 0x1p-10f && temperature <= 0x1p10f) || (top > 0 && (!tid || !tlog)))
+namespace {
+// What a call says, in the order of functional.py's _LOSS_CALL.  Outer index i of an array lies at (i / cols) * s0 + (i % cols) * s1.
+struct LossCall {
+  int mode, dtype;                                    // mode: 1 loss and stats, 2 gradient from stats, 3 loss and gradient; 0 fp16, 1 bf16, 2 fp32
+  const void* logits;
+  long long ld;
+  int rows, V;
+  const void* labels;                                 // null: none
+  int labels64, label_cols;
+  long long label_s0, label_s1, ignore;
+  const void* tid;                                    // null: no teacher
+  int tid64, tid_cols;
+  long long tid_s0, tid_s1;
+  const void* tlog;
+  int tlog_dtype, tlog_cols;
+  long long tlog_s0, tlog_s1;
+  int top;
+  float temperature, weight, grad_scale;
+  float *loss, *stats;
+  void* dlogits;                                      // may be logits
+  long long ldd;
+  const float* grad_loss;
+  long long ldg;
+  int* status;
+};
+static_assert(sizeof(LossCall) == 208, "the size of _LOSS_CALL");
+}  // namespace
+
+// The call is one piece of memory (of `bytes`, for a check): 34 arguments by themselves take ctypes 4 us.
+extern "C" int tp_loss(const void* call, int bytes, void* stream) {
+  if (!call || bytes != static_cast<int>(sizeof(LossCall))) return kErrBadArgument;
+  const LossCall& c = *static_cast<const LossCall*>(call);
+  if (c.mode < 1 || c.mode > 3 || c.dtype < 0 || c.dtype > 2 || c.tlog_dtype < 0 || c.tlog_dtype > 2 || c.rows < 0 || c.V < 0 || c.top < 0 ||
+      c.label_cols < 1 || c.tid_cols < 1 || c.tlog_cols < 1 || !(c.temperature >= 0x1p-10f && c.temperature <= 0x1p10f) ||
+      !(c.weight >= 0.0f && c.weight <= 1.0f) || (c.top > 0 && (!c.tid || !c.tlog)))
     return kErrBadArgument;
-  if (top > kMaxTop) return kErrTooLarge;
-  if (rows == 0) return kOk;
-  if (((mode & kLossFwd) && !loss) || (mode == kLossBwd && !stats) || ((mode & kLossBwd) && V > 0 && !dlogits))
+  if (c.top > kMaxTop) return kErrTooLarge;
+  if (c.rows == 0) return kOk;
+  if (((c.mode & kLossFwd) && !c.loss) || (c.mode == kLossBwd && !c.stats) || ((c.mode & kLossBwd) && c.V > 0 && !c.dlogits))
     return kErrBadArgument;
-  LossArgs a{logits, ld, rows, V, labels, OuterIndex{label_s0, label_s1, label_cols}, ignore, labels64, tid, tlog,
-             OuterIndex{tid_s0, tid_s1, tid_cols}, OuterIndex{tlog_s0, tlog_s1, tlog_cols}, top, tid64, tlog_dtype,
-             temperature, weight, loss, stats, dlogits, ldd, grad_loss, ldg, grad_scale, status};
+  LossArgs a{c.logits, c.ld, c.rows, c.V, c.labels, OuterIndex{c.label_s0, c.label_s1, c.label_cols}, c.ignore, c.labels64, c.tid, c.tlog,
+             OuterIndex{c.tid_s0, c.tid_s1, c.tid_cols}, OuterIndex{c.tlog_s0, c.tlog_s1, c.tlog_cols}, c.top, c.tid64, c.tlog_dtype,
+             c.temperature, c.weight, c.loss, c.stats, c.dlogits, c.ldd, c.grad_loss, c.ldg, c.grad_scale, c.status};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == 0) return loss_launch_fp16(a, mode, s);
-  if (dtype == 1) return loss_launch_bf16(a, mode, s);
-  return loss_launch_fp32(a, mode, s);
+  if (c.dtype == 0) return loss_launch_fp16(a, c.mode, s);
+  if (c.dtype == 1) return loss_launch_bf16(a, c.mode, s);
+  return loss_launch_fp32(a, c.mode, s);
 }

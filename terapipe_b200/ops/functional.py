@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Optional
 
 import torch
@@ -276,6 +277,7 @@ _DT_IDS = {torch.int32: 0, torch.int64: 1}
 MAX_TEACHER_ENTRIES = 1024
 
 
+# (What a call costs on the host counts for small ones: sizes and strides are looked at once, the common cases first.)
 def _kind(t: torch.Tensor, kinds, what: str) -> int:
     code = kinds.get(t.dtype)
     if code is None:
@@ -296,6 +298,8 @@ def _outer(t: torch.Tensor, inner: int, n: int, what: str):
     two dimensions with any strides (a batch-first array seen sequence-first), or of more that a view can join."""
     shape, st = t.shape, t.stride()
     d = len(shape) - inner
+    if d == 1 and shape[0] == n:
+        return 1, st[0], 0
     if d < 0 or math.prod(shape[:d]) != n:
         raise KernelError(f"{what} {tuple(shape)} does not have {n} rows")
     if n <= 1:
@@ -324,12 +328,16 @@ def _matrix(t: torch.Tensor, what: str):
     shape, st = t.shape, t.stride()
     if not shape:
         raise KernelError(f"{what} is a scalar")
-    rows, ld = (shape[0], st[0]) if len(shape) == 2 else _joined(shape, st, len(shape) - 1, what)
-    if st[-1] != 1 and shape[-1] > 1:
+    if len(shape) == 2:
+        (rows, cols), ld = shape, st[0]
+    else:
+        cols = shape[-1]
+        rows, ld = _joined(shape, st, len(shape) - 1, what)
+    if st[-1] != 1 and cols > 1:
         raise KernelError(f"{what}: columns are contiguous, not {st[-1]} apart")
-    if rows >= 2 ** 31 or shape[-1] >= 2 ** 31:
-        raise KernelError(f"{what}: {rows} rows of {shape[-1]} columns are too many")
-    return rows, shape[-1], ld
+    if rows >= 2 ** 31 or cols >= 2 ** 31:
+        raise KernelError(f"{what}: {rows} rows of {cols} columns are too many")
+    return rows, cols, ld
 
 
 def _written(t: torch.Tensor, rows: int, cols: int, ld: int, what: str) -> None:
@@ -400,17 +408,25 @@ def embedding_bwd(ids, dy, dweight, *, scale: float = 1.0, first_row: int = 0, p
     return dweight
 
 
+# tp_loss's arguments as one piece of memory (LossCall in csrc/loss.cu): 34 of them by themselves take ctypes 4 us
+_LOSS_CALL = struct.Struct("iiPqiiPiiqqqPiiqqPiiqqifffPPPqPqP")
+_NO_LABELS = (0, 0, 1, 0, 0, 0)
+_NO_TEACHER = (0, 0, 1, 0, 0, 0, 0, 1, 0, 0, 0)
+
+
 def _loss(mode, logits, teacher, labels, temperature, teacher_weight, ignore_id, loss=None, stats=None, dlogits=None,
           grad_loss=None, grad_scale=1.0):
     n, V, ld = _matrix(logits, "logits")
     dtype = _kind(logits, _DT_ROWS, "logits")
-    label_args = (None, 0, 1, 0, 0, 0)
+    dev, p = logits.get_device(), logits.data_ptr()
+    away = dev != torch._C._cuda_getDevice()
+    label_args, teacher_args = _NO_LABELS, _NO_TEACHER
     if labels is not None:
+        away |= labels.get_device() != dev
         label_args = (labels.data_ptr(), _kind(labels, _DT_IDS, "labels"), *_outer(labels, 0, n, "labels"), ignore_id)
-    teacher_args = (None, 0, 1, 0, 0, None, 0, 1, 0, 0, 0)
-    tid = tlog = None
     if teacher is not None:
         tid, tlog = teacher
+        away |= tid.get_device() != dev or tlog.get_device() != dev
         if tid.shape != tlog.shape or tid.dim() < 2:
             raise KernelError(f"teacher ids {tuple(tid.shape)} and logits {tuple(tlog.shape)}: [..., entries] of one shape")
         top = tid.shape[-1]
@@ -418,20 +434,25 @@ def _loss(mode, logits, teacher, labels, temperature, teacher_weight, ignore_id,
             raise KernelError(f"{top} teacher entries a row; at most {MAX_TEACHER_ENTRIES}")
         if top > 1 and (tid.stride(-1) != 1 or tlog.stride(-1) != 1):
             raise KernelError("a row's teacher entries are contiguous")
-        teacher_args = (tid.data_ptr(), _kind(tid, _DT_IDS, "teacher ids"), *_outer(tid, 1, n, "teacher ids"),
-                        tlog.data_ptr(), _kind(tlog, _DT_ROWS, "teacher logits"), *_outer(tlog, 1, n, "teacher logits"), top)
         if not 2 ** -10 <= temperature <= 2 ** 10 or not 0 <= teacher_weight <= 1:
             raise KernelError(f"temperature {temperature} in [2^-10, 2^10] and teacher_weight {teacher_weight} in [0, 1]")
+        teacher_args = (tid.data_ptr(), _kind(tid, _DT_IDS, "teacher ids"), *_outer(tid, 1, n, "teacher ids"),
+                        tlog.data_ptr(), _kind(tlog, _DT_ROWS, "teacher logits"), *_outer(tlog, 1, n, "teacher logits"), top)
+    loss_ptr = stats_ptr = out_ptr = grad_ptr = 0
     if mode & 1:
         if loss is None:
             loss = torch.empty(n, dtype=torch.float32, device=logits.device)
         elif loss.dtype != torch.float32 or loss.numel() != n or not loss.is_contiguous():
             raise KernelError(f"loss is float32 [{n}], contiguous")
+        away |= loss.get_device() != dev
+        loss_ptr = loss.data_ptr()
     if mode == 1 and stats is None:
         stats = torch.empty(n, 8, dtype=torch.float32, device=logits.device)
-    elif stats is not None and (stats.dtype != torch.float32 or stats.numel() != 8 * n or not stats.is_contiguous()
-                                or stats.data_ptr() % 16):
-        raise KernelError(f"stats is float32 [{n}, 8], contiguous on a 16-byte boundary")
+    if stats is not None:
+        stats_ptr = stats.data_ptr()
+        if stats.dtype != torch.float32 or stats.numel() != 8 * n or not stats.is_contiguous() or stats_ptr % 16:
+            raise KernelError(f"stats is float32 [{n}, 8], contiguous on a 16-byte boundary")
+        away |= stats.get_device() != dev
     ldd = ldg = 0
     if mode & 2:
         if dlogits is None:
@@ -440,10 +461,13 @@ def _loss(mode, logits, teacher, labels, temperature, teacher_weight, ignore_id,
         if n_d != n or V_d != V or dlogits.dtype != logits.dtype:
             raise KernelError(f"dlogits {tuple(dlogits.shape)} {dlogits.dtype} for logits {tuple(logits.shape)} {logits.dtype}")
         _written(dlogits, n, V, ldd, "dlogits")
+        away |= dlogits.get_device() != dev
+        out_ptr = dlogits.data_ptr()
         if n and V:
             # in place, or apart: a row's gradient is stored while other rows' logits are still to be read
-            p, q, es = logits.data_ptr(), dlogits.data_ptr(), logits.element_size()
-            if (p != q or (ld != ldd and n > 1)) and p < q + ((n - 1) * ldd + V) * es and q < p + ((n - 1) * ld + V) * es:
+            es = logits.element_size()
+            if (p != out_ptr or (ld != ldd and n > 1)) and p < out_ptr + ((n - 1) * ldd + V) * es \
+                    and out_ptr < p + ((n - 1) * ld + V) * es:
                 raise KernelError("dlogits is logits itself or does not overlap it")
         if grad_loss is not None:
             if grad_loss.dtype != torch.float32:
@@ -451,10 +475,13 @@ def _loss(mode, logits, teacher, labels, temperature, teacher_weight, ignore_id,
             n_g, ldg = _joined(grad_loss.shape, grad_loss.stride(), grad_loss.dim(), "grad_loss")
             if n_g != n:
                 raise KernelError(f"grad_loss {tuple(grad_loss.shape)} does not have {n} rows")
-    _same_device(logits, labels, tid, tlog, loss, stats, dlogits, grad_loss)
-    st = cuda_lib().tp_loss(mode, dtype, logits.data_ptr(), ld, n, V, *label_args, *teacher_args, temperature,
-                            teacher_weight, _ptr(loss), _ptr(stats), _ptr(dlogits), ldd, _ptr(grad_loss), ldg, grad_scale,
-                            _status_ptr(logits), _stream())
+            away |= grad_loss.get_device() != dev
+            grad_ptr = grad_loss.data_ptr()
+    if away:
+        raise KernelError("tensors of the current device")
+    call = _LOSS_CALL.pack(mode, dtype, p, ld, n, V, *label_args, *teacher_args, temperature, teacher_weight, grad_scale, loss_ptr,
+                           stats_ptr, out_ptr, ldd, grad_ptr, ldg, _status_ptr(logits))
+    st = cuda_lib().tp_loss(call, len(call), _stream())
     if st:
         check(st, "tp_loss")
     return loss, stats, dlogits

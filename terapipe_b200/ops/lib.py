@@ -130,7 +130,7 @@ SIGNATURES = {
     "tp_embedding_fwd": [I, P, I, I, I, L, L, L, P, L, L, P, L, I, F, P],
     "tp_embedding_bwd_workspace_blocks": [I, L, I],
     "tp_embedding_bwd": [I, P, I, I, I, L, L, L, L, P, L, P, L, L, I, F, I, P, P],
-    "tp_loss": [I, I, P, L, I, I, P, I, I, L, L, L, P, I, I, L, L, P, I, I, L, L, I, F, F, P, P, P, L, P, L, F, P, P],
+    "tp_loss": [P, I, P],
     "tp_attn_bwd_scaled": [I, I, F, P, I, I, I, I, I, P, L, P, L, P, L, P, P, L, P, P],
 }
 
