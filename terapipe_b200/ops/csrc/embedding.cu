@@ -516,7 +516,8 @@ static int key_bits(long long rows) {   // keys are 0 .. rows
   return bits;
 }
 
-// Tokens a warp sums: 32 where that leaves 32 warps for every SM, else 8.  5105 tokens of 1600 columns: PIECE8 us against PIECE32.
+// Tokens a warp sums: 32 where that leaves 32 warps for every SM, else 8.  Added to a gradient, us with 8 / 32 tokens
+// a warp: 600 tokens of 1600 columns 27 / 32, 5105 29.5 / 35.6, 16384 of 2048 52 / 54, 147456 342 / 284.
 static int sum_piece(int n, int H) { return static_cast<long long>(n) * ((H + 255) / 256) >= 32ll * 32 * num_sms() ? 32 : 8; }
 
 

@@ -43,9 +43,10 @@ extern "C" int tp_loss(const void* call, int bytes, void* stream) {
   if (c.rows == 0) return kOk;
   if (((c.mode & kLossFwd) && !c.loss) || (c.mode == kLossBwd && !c.stats) || ((c.mode & kLossBwd) && c.V > 0 && !c.dlogits))
     return kErrBadArgument;
+  const float temperature = c.top > 0 ? c.temperature : 1.0f;      // the label's term has none
   LossArgs a{c.logits, c.ld, c.rows, c.V, c.labels, OuterIndex{c.label_s0, c.label_s1, c.label_cols}, c.ignore, c.labels64, c.tid, c.tlog,
              OuterIndex{c.tid_s0, c.tid_s1, c.tid_cols}, OuterIndex{c.tlog_s0, c.tlog_s1, c.tlog_cols}, c.top, c.tid64, c.tlog_dtype,
-             c.temperature, c.weight, c.loss, c.stats, c.dlogits, c.ldd, c.grad_loss, c.ldg, c.grad_scale, c.status};
+             temperature, c.weight, c.loss, c.stats, c.dlogits, c.ldd, c.grad_loss, c.ldg, c.grad_scale, c.status};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (c.dtype == 0) return loss_launch_fp16(a, c.mode, s);
   if (c.dtype == 1) return loss_launch_bf16(a, c.mode, s);

@@ -268,15 +268,6 @@ __device__ __forceinline__ PartOfRow load_part(uint32_t cluster_addr) {
                : "=f"(p.mass), "=f"(p.zy), "=f"(p.own), "=f"(p.pad) : "r"(cluster_addr + 16) : "memory");
   return p;
 }
-// Stores a part into another CTA's shared memory; its bytes count on that CTA's barrier.  (A cluster barrier would do as
-// well, but its release waits for all of the CTA's stores to global memory, a row's gradient each time.)
-__device__ __forceinline__ void send_part(const PartOfRow& p, uint32_t cluster_addr, uint32_t cluster_bar) {
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];"
-               ::"r"(cluster_addr), "f"(p.m), "f"(p.s1), "f"(p.st), "f"(p.dot), "r"(cluster_bar) : "memory");
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];"
-               ::"r"(cluster_addr + 16), "f"(p.mass), "f"(p.zy), "f"(p.own), "f"(p.pad), "r"(cluster_bar) : "memory");
-}
-
 // t_max: largest of the teacher's logits (0 where there is none), t_sum: sum of exp((t - t_max) / T) over the entries, entropy: the same
 // weighted with (t - t_max) / T.  stats: largest logit (0 where all are -inf), sums of exp(z - largest) and of
 // exp((z - largest) / T), t_max, t_sum.
@@ -313,14 +304,6 @@ __device__ __forceinline__ void store_entry(T* out, int id, int k, float e1, flo
   if (id != label) g1 = 0.0f;
   // (with DUAL each difference by itself: exactly zero where both distributions have one value only)
   out[id] = Elem<T>::from_f(DUAL ? (c1 * e1 - g1) + (ct * et - gp * p) : c1 * e1 - (g1 + gp * p));
-}
-
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int LEFT> __device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
 }
 
 // ------------------------------------------------------------------ rows held on chip
@@ -931,7 +914,7 @@ loss_stream_kernel(const LossArgs a, int parts, int per) {
 // ------------------------------------------------------------------ the gradient from a forward pass's statistics
 // A CTA per part of a row, four granules a thread.  Bound by the bytes; what a row needs besides is on its way together with its
 // logits.  (With the sums of the forward kernel's kind over the teacher's entries before the logits were asked for, 2045 rows of
-// 32000 fp32 logits took 207 us, FAST this way; of 16384 rows of 2000, 512 threads each, 164 and SMALL.)
+// 32000 fp32 logits took 207 us, 120 this way; 16384 rows of 2000 bf16, 512 threads each, 164 and 33.)
 template <typename T, int SOFT, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 loss_bwd_kernel(const LossArgs a, int parts, int table) {

@@ -285,6 +285,22 @@ def test_no_rows_and_no_columns():
     assert (loss == 0).all() and (grad == 0).all()
 
 
+def test_labels_beside_a_teacher_without_entries():
+    """No room for entries at all: the label's term alone, at a temperature of 1."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    z, labels = _logits(20, 3001, torch.float16, g), torch.randint(0, 3001, (20,), device="cuda", generator=g)
+    none = torch.empty(20, 0, dtype=torch.int64, device="cuda"), torch.empty(20, 0, device="cuda")
+    from terapipe_b200.ops import functional as F
+    how = {"temperature": 2.0, "teacher_weight": 0.25}
+    loss64, grad64 = _formula(z, None, None, labels, 1.0, 0.25)
+    loss, grad = F.distill_fwd_bwd(z, *none, labels, **how)
+    loss2, stats = F.distill_fwd(z, *none, labels, **how)
+    grad2 = F.distill_bwd(z, stats, *none, labels, **how)
+    for a, b in ((loss, grad), (loss2, grad2)):
+        assert ((a.double() - loss64).abs() <= 2.0 ** -20 * 40).all()
+        assert ((b.double() - grad64).abs() <= 2.0 ** -11 * grad64.abs() + 2.0 ** -18).all()
+
+
 def test_rows_beyond_32_bit_offsets():
     """The last rows of a matrix of more than 2^32 elements."""
     from terapipe_b200.ops import functional as F
