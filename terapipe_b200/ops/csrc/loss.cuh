@@ -336,8 +336,11 @@ struct alignas(16) RowKnown {
   float m, c1, ct;     // largest logit; factors of exponentials relative to it
   int active;          // 0: the gradient is zero
 };
-// What is known of a row before its sums: its label and entries.
-struct RowTerms {
+// What is known of a row before its sums: its label and entries.  The factors that its sums are divided into come first.
+struct alignas(16) RowTerms {
+  float f1, ft;                     // of the two exponentials, or of the one (f1)
+  int active;                       // the row has a term
+  int pad;
   float g, zy, t_max, t_sum, entropy;      // the row's factor; z_y if the label is in this part; of all entries
   int label, listed;                // -1: no label; entries listed
   bool teach, own, twice;           // the row has the teacher's term; the label is in this part; an id occurs twice in it
@@ -563,21 +566,29 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
     bool ok = true;
     for (int row = row0, buf = 0, turn = 0; row < a.rows; row += stride, z += z_step, out += out_step, buf ^= 1, turn ^= buf == 0, ++n) {
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(&parts_in[buf], turn, wait, kErrWaitPeer)))) break;
+      // (what stands between the last warp's sums and `known` is all of the row's chain that no other warp overlaps: nothing more here)
       float m = -INFINITY, s1 = 0.0f, st = 0.0f;
-      for (int i = lane; i < senders; i += 32) m = fmaxf(m, inbox[buf][i].m);
-      m = warp_max(m);
-      if (m == -INFINITY) m = 0.0f;
-      for (int i = lane; i < senders; i += 32) {
-        const WarpPart p = inbox[buf][i];
-        s1 += p.s1 * Exponent{k1, m}.factor(p.m);
-        if (DUAL) st += p.st * Exponent{kt, m}.factor(p.m);
+      if (senders <= 32) {
+        const WarpPart p = lane < senders ? inbox[buf][lane] : WarpPart{-INFINITY, 0.0f, 0.0f, 0.0f};
+        m = warp_max(p.m);
+        if (m == -INFINITY) m = 0.0f;
+        s1 = p.s1 * Exponent{k1, m}.factor(p.m);
+        if (DUAL) st = p.st * Exponent{kt, m}.factor(p.m);
+      } else {
+        for (int i = lane; i < senders; i += 32) m = fmaxf(m, inbox[buf][i].m);
+        m = warp_max(m);
+        if (m == -INFINITY) m = 0.0f;
+        for (int i = lane; i < senders; i += 32) {
+          const WarpPart p = inbox[buf][i];
+          s1 += p.s1 * Exponent{k1, m}.factor(p.m);
+          if (DUAL) st += p.st * Exponent{kt, m}.factor(p.m);
+        }
       }
+      const float f1 = terms[n & 3].f1, ft = terms[n & 3].ft;
       s1 = warp_add(s1);
       st = DUAL ? warp_add(st) : s1;
-      const RowTerms t = terms[n & 3];
-      const RowFactors f(a, t.g, t.label >= 0, t.teach);
-      const float c1 = (DUAL ? f.g1 : f.g1 + f.gt) * (1.0f / s1), ct = DUAL ? f.gt * (1.0f / st) : 0.0f;
-      const bool active = (t.label >= 0 || t.teach) && s1 != 0.0f;
+      const float c1 = f1 * (1.0f / s1), ct = DUAL ? ft * (1.0f / st) : 0.0f;
+      const bool active = terms[n & 3].active && s1 != 0.0f;
       if (lane == 0) {
         known_row[buf] = RowKnown{m, c1, ct, active};
         mbar_arrive(&known[buf]);
@@ -586,6 +597,8 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
       if (row + 2 * stride < a.rows) fetch(z + 2 * z_step, buf, edge[2]);
       if (row + 3 * stride < a.rows) edge[3] = load_edge(z + 3 * z_step);
       if (rank == 0 && n > 0 && !(ok = finish_loss(row - stride, n - 1))) break;
+      const RowTerms t = terms[n & 3];
+      const RowFactors f(a, t.g, t.label >= 0, t.teach);
       const float* list_p = list_p_all + (n & 3) * a.top;
       const float* list_z = list_z_all + (n & 3) * a.top;
       const int* list_id = list_id_all + (n & 3) * a.top;
@@ -660,7 +673,7 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
       float* list_p = list_p_all + (n & 3) * a.top;
       float* list_z = list_z_all + (n & 3) * a.top;
       int* list_id = list_id_all + (n & 3) * a.top;
-      RowTerms now{raw_g, 0.0f, 0.0f, 0.0f, 0.0f, raw_label.get(a), 0, false, false, false};
+      RowTerms now{0.0f, 0.0f, 0, 0, raw_g, 0.0f, 0.0f, 0.0f, 0.0f, raw_label.get(a), 0, false, false, false};
       float t_max = -INFINITY;
       for (int k0 = 0; k0 < a.top; k0 += 32 * kAhead) {
         if (k0 > 0) load_entries<kAhead>(a, row, k0 + lane, raw_entry);
@@ -722,6 +735,10 @@ loss_rows_kernel(const LossArgs a, int parts, int per, int table) {
         now.twice = __any_sync(0xffffffffu, mine);
       }
       now.teach = a.weight != 0.0f && now.t_sum != 0.0f;
+      now.active = now.label >= 0 || now.teach;
+      const RowFactors f(a, now.g, now.label >= 0, now.teach);
+      now.f1 = DUAL ? f.g1 : f.g1 + f.gt;
+      now.ft = f.gt;
       if (rank == 0) now.entropy = warp_add(now.entropy);
       __syncwarp();
       if (lane == 0) {
@@ -940,7 +957,7 @@ loss_bwd_kernel(const LossArgs a, int parts, int table) {
   }
   RawLabel raw_label{};
   raw_label.load(a, row);
-  const float4 s0 = reinterpret_cast<const float4*>(a.stats)[2 * row];
+  const float4 s0 = reinterpret_cast<const float4*>(a.stats)[2ll * row];
   const float t_max = s0.w, t_sum = a.stats[8ll * row + 4], g = a.grad_loss ? a.grad_loss[row * a.ldg] : 1.0f;
 #pragma unroll
   for (int k = 0; k < kNG; ++k) {
