@@ -320,6 +320,10 @@ __device__ __forceinline__ void store_entry(T* out, int id, int k, float e1, flo
 // sums of all warps of the cluster have arrived, by st.async where it has several CTAs, and the row's terms are known), `known`
 // (they are added up), `written` (the CTA's part of the gradient is stored).  The label's and the teacher's elements of the
 // gradient are then stored again, while the threads are on the next row.
+//
+// Measured for 4096 rows with their gradient: 50304 bf16 logits and a label 156 us (5.3 TB/s of the 6.56 that a copy reaches),
+// with 64 entries of a teacher 161; 131072 bf16 logits 414; 32000 fp32 logits 200.  Without the gradient, 50304 bf16: 97.
+// Taking in all of a row's terms before `known`, and not two factors made beforehand, cost 10 of the 156.
 
 // CTAs an SM has registers for, by the exponentials a thread keeps.
 constexpr int loss_ctas_per_sm(int threads, int values) {
