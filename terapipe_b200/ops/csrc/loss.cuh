@@ -323,7 +323,7 @@ __device__ __forceinline__ void store_entry(T* out, int id, int k, float e1, flo
 //
 // Measured for 4096 rows with their gradient: 50304 bf16 logits and a label 156 us (5.3 TB/s of the 6.56 that a copy reaches),
 // with 64 entries of a teacher 161; 131072 bf16 logits 414; 32000 fp32 logits 200.  Without the gradient, 50304 bf16: 97.
-// Taking in all of a row's terms before `known`, and not two factors made beforehand, cost 10 of the 156.
+// (The first took 165 with all of a row's terms taken in before `known`, and not two factors made beforehand.)
 
 // CTAs an SM has registers for, by the exponentials a thread keeps.
 constexpr int loss_ctas_per_sm(int threads, int values) {
